@@ -44,6 +44,20 @@ SYMBOLS = [
     ("b200q_gemm_static_max_bytes", _sz, []),
     ("b200q_gemm_static", _i, [_i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp]),
     ("b200q_linear", _i, [_i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _vp]),
+    ("b200q_mx4_image_bytes", _sz, [_i64, _i]),
+    ("b200q_mx4_pack", _i, [_vp, _i64, _i64, _i, _vp, _vp]),
+    ("b200q_mx4_quantize", _i, [_vp, _i, _i64, _i, _vp, _vp]),
+    ("b200q_mx4_dequantize", _i, [_vp, _i64, _i, _vp, _i, _vp]),
+    ("b200q_mx4_gemm", _i, [_vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp]),
+    ("b200q_mx4_linear_workspace_bytes", _sz, [_i, _i]),
+    ("b200q_mx4_linear", _i, [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _vp]),
+    ("b200q_moe_plan_bytes", _sz, [_i64, _i, _i]),
+    ("b200q_moe_plan", _i, [_vp, _i64, _i, _i, _vp, _vp]),
+    ("b200q_moe_route", _i, [_vp, _i, _i64, _i, _i, _i, C.c_float, _vp, _vp, _vp, _vp]),
+    ("b200q_moe_mx4_workspace_bytes", _sz, [_i64, _i, _i, _i]),
+    ("b200q_moe_mx4_linear", _i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _i, _vp, _sz, _vp]),
+    ("b200q_moe_mx4_swiglu", _i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _i, _i64, _i, _i, _i, _i, _vp, _sz, _vp]),
+    ("b200q_moe_combine", _i, [_vp, _i, _vp, _vp, _i64, _i, _i, _i, _vp, _vp]),
     ("b200q_tc_calls_consume", C.c_ulonglong, [_i]),
     ("brotensor_q4k_wmma_calls_consume", C.c_ulonglong, []),
     ("brotensor_q6k_wmma_calls_consume", C.c_ulonglong, []),

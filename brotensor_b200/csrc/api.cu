@@ -123,6 +123,15 @@ static int dev_info(DevInfo** out) {
     return B200Q_OK;
 }
 
+// The current device's SM count and status word, for the entry points of api_mx4.cu.
+int device_facts(int* sms, int** status) {
+    DevInfo* d;
+    if (int rc = dev_info(&d)) return rc;
+    *sms = d->sms;
+    *status = d->status;
+    return B200Q_OK;
+}
+
 int* device_status_word(int dev) { return (dev >= 0 && dev < kMaxDev && g_dev[dev].ready.load(std::memory_order_acquire)) ? g_dev[dev].status : nullptr; }
 
 // Which kernel the thread's last linear call went to (option "last_kernel"): tests ask, since every route gives nearly the same numbers.

@@ -259,6 +259,70 @@ int b200q_linear(int fmt, const void* W, const void* X, int x_dtype, const void*
                  int M, int N, int K, void* ws, size_t ws_bytes, void* stream);
 
 /*
+ * MXFP4 matrices (OCP Microscaling Formats 1.0): 32 neighbouring elements of a row share a scale 2^(e - 127), an
+ * element is 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with a sign. On the device such a matrix is an "image" of b200q_mx4_image_bytes() bytes, in the
+ * operand layout of the block-scaled tensor cores; its inner layout is the library's own. K is a multiple of 32 (columns up to the
+ * next multiple of 256 are kept as zeros); rows beyond the last of a tile of 128 are not specified. Images are
+ * 16-byte aligned. brotensor's loader does not know the format.
+ *
+ * b200q_mx4_pack       a file's blocks (ggml block_mxfp4: u8 e, u8 qs[16]; element j < 16 the low nibble of qs[j], else the high nibble
+ *                      of qs[j - 16]; 17 bytes, any alignment) -> image, bit for bit. `count` matrices of rows x K, one after the other in
+ *                      `blocks`, each get an image of their own, b200q_mx4_image_bytes(rows, K) apart (the experts of a layer).
+ * b200q_mx4_quantize   rows x K of x_dtype -> image. e - 127 = floor(log2(largest magnitude of the block)) - 2, at least -127;
+ *                      elements are rounded to the nearest value, ties to the even one, magnitudes beyond 6 to 6. A block that holds an
+ *                      infinity or a NaN reads back as NaN.
+ * b200q_mx4_dequantize image -> rows x K of out_dtype, 16-byte aligned: the values, rounded once where the type does not hold them.
+ *
+ * b200q_mx4_gemm       Y(M,N) = X(M,K) W(N,K)^T (+ bias(N)) of two images: exact products, FP32 sums on the tensor cores, one rounding to
+ *                      y_dtype. Any M >= 0; few output tiles have K split over a cluster's CTAs, with a fixed order of the sums: the
+ *                      result does not change from run to run.
+ * b200q_mx4_linear     the same from X of x_dtype, quantised into `ws` (b200q_mx4_linear_workspace_bytes(M, K) bytes, 256-byte aligned; a
+ *                      larger one will do) on the way; bias is of x_dtype. Calls that share a workspace must be ordered on one stream.
+ */
+size_t b200q_mx4_image_bytes(int64_t rows, int K); /* 0 if K is not a positive multiple of 32 */
+int b200q_mx4_pack(const void* blocks, int64_t count, int64_t rows, int K, void* image, void* stream);
+int b200q_mx4_quantize(const void* x, int x_dtype, int64_t rows, int K, void* image, void* stream);
+int b200q_mx4_dequantize(const void* image, int64_t rows, int K, void* out, int out_dtype, void* stream);
+int b200q_mx4_gemm(const void* W, const void* X_image, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K,
+                   void* stream);
+size_t b200q_mx4_linear_workspace_bytes(int M, int K);
+int b200q_mx4_linear(const void* W, const void* X, int x_dtype, const void* bias, void* Y, int y_dtype, int M, int N, int K, void* ws,
+                     size_t ws_bytes, void* stream);
+
+/*
+ * Sparse expert layers: each token goes through k of E experts (1 <= E <= 1024, 1 <= k <= 32). Pair s = t * k + j is token t's j-th choice.
+ *
+ * b200q_moe_route      logits: tokens x E of dtype. ids (tokens x k): the k experts with the largest logits, largest first, ties to the
+ *                      lower expert; weights (tokens x k, FP32): scale * exp(l) / sum of exp(l) over the chosen (normalize != 0) or over
+ *                      all experts. Logits of -inf or NaN are never chosen: a token that runs out of experts gets id -1 and weight 0. An infinite
+ *                      logit takes all the weight (equal shares of several). `plan`, where not NULL, is b200q_moe_plan of the ids.
+ * b200q_moe_plan       the pairs grouped by expert, for ids from anywhere: int32 `plan` of b200q_moe_plan_bytes() bytes, 16-byte aligned.
+ *                      It begins with offsets[E + 1] - expert e has places offsets[e] .. offsets[e + 1] - 1 - and order[tokens * k], the
+ *                      pair of each place; the pairs of an expert keep their order, and places from offsets[E] on hold -1. The rest is the
+ *                      library's own. An id outside 0 .. E - 1 is no expert; the same expert may come twice in a token.
+ * b200q_moe_mx4_linear Y(pair, N) = quantise(X row) W_e(N,K)^T (+ bias_e(N)), e the pair's expert. W: E images of N x K, one
+ *                      after the other (b200q_mx4_pack with count = E); X: tokens x K, a row for all pairs of its token, or with x_per_pair
+ *                      tokens * k x K; bias: E x N of x_dtype or NULL; Y: tokens * k rows of N. Rows of pairs without an expert
+ *                      are left as they were. `plan` must be of the same tokens, k and E. `ws`: b200q_moe_mx4_workspace_bytes() bytes,
+ *                      256-byte aligned, shared only by calls that are ordered on one stream.
+ * b200q_moe_mx4_swiglu Y(pair, N) = silu(gate) * up of two such products, silu(v) = v / (1 + exp(-v)), without writing them out.
+ * b200q_moe_combine    out(t, N) = sum over j of weights[t][j] * y(t, j, N), in the order of j in FP32; y and out of dtype. Pairs whose id
+ *                      is outside 0 .. E - 1 are not read.
+ * Nothing depends on values that would have to be read back: a layer's calls can be captured in a graph and replayed with other ids.
+ */
+size_t b200q_moe_plan_bytes(int64_t tokens, int k, int E); /* 0 outside the supported sizes */
+int b200q_moe_plan(const int32_t* ids, int64_t tokens, int k, int E, void* plan, void* stream);
+int b200q_moe_route(const void* logits, int dtype, int64_t tokens, int E, int k, int normalize, float scale, int32_t* ids, float* weights,
+                    void* plan, void* stream);
+size_t b200q_moe_mx4_workspace_bytes(int64_t tokens, int k, int E, int K);
+int b200q_moe_mx4_linear(const void* W, const void* X, int x_dtype, int x_per_pair, const void* plan, const void* bias, void* Y, int y_dtype,
+                         int64_t tokens, int k, int E, int N, int K, void* ws, size_t ws_bytes, void* stream);
+int b200q_moe_mx4_swiglu(const void* W_gate, const void* W_up, const void* X, int x_dtype, int x_per_pair, const void* plan, void* Y,
+                         int y_dtype, int64_t tokens, int k, int E, int N, int K, void* ws, size_t ws_bytes, void* stream);
+int b200q_moe_combine(const void* y, int dtype, const int32_t* ids, const float* weights, int64_t tokens, int k, int E, int N, void* out,
+                      void* stream);
+
+/*
  * How many tensor-core GEMM launches were made for `fmt` on this thread's
  * device since the last call; reading resets the count. The three named
  * aliases are the hooks brotensor's parity tests link against
