@@ -52,6 +52,8 @@ size_t gemm_mm_workspace_bytes(int fmt, int x_dtype, int M, int N, int K);
 int launch_gemm_mm(int fmt, const void* W, const void* X, int x_dtype, const void* bias, void* Y, int y_dtype, int M, int N, int K,
                    void* ws, size_t ws_bytes, int sms, cudaStream_t st, bool* taken);
 void mm_set_enabled(int v);
+void mx4_set_wide(int v);
+int mx4_get_wide();
 int mm_get_enabled();
 int mb_get_enabled();
 void i8_set_enabled(int v);
@@ -632,6 +634,7 @@ int b200q_set_option(const char* key, int value) {
     else if (!strcmp(key, "gemv_mb")) mb_set_enabled(value);
     else if (!strcmp(key, "gemv_hm")) hm_set_enabled(value);
     else if (!strcmp(key, "gemm_mm")) mm_set_enabled(value);
+    else if (!strcmp(key, "mx4_wide")) mx4_set_wide(value);
     else if (!strcmp(key, "gemv_step_fill")) dp_set_step_fill(value);
     else return fail(B200Q_ERR_BAD_ARG, "set_option: unknown key '%s'", key);
     return B200Q_OK;
@@ -650,6 +653,7 @@ int b200q_get_option(const char* key, int* out) {
     else if (!strcmp(key, "gemv_mb")) *out = mb_get_enabled();
     else if (!strcmp(key, "gemv_hm")) *out = hm_get_enabled();
     else if (!strcmp(key, "gemm_mm")) *out = mm_get_enabled();
+    else if (!strcmp(key, "mx4_wide")) *out = mx4_get_wide();
     else if (!strcmp(key, "gemv_tile_pairs")) *out = dp_get_tile_pairs();
     else if (!strcmp(key, "gemm_pair")) *out = gemm_get_pair();
     else if (!strcmp(key, "gemm_split")) *out = gemm_get_split();

@@ -62,6 +62,88 @@ __device__ __forceinline__ float e2m1_to_f32(uint32_t nib) {
 __device__ __forceinline__ size_t mx_tile_offset(int64_t row_tile, int k_tile, int k_tiles) { return ((size_t)row_tile * k_tiles + k_tile) * kMxTileBytes; }
 __device__ __forceinline__ uint32_t mx_chunk_offset(int r, int b) { return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((b ^ (r & 7)) << 4)); }
 __device__ __forceinline__ uint32_t mx_scale_offset(int r, int half) { return (uint32_t)(kMxQBytes + half * 512 + (r & 31) * 16 + (r >> 5) * 4); }
+// ---- tcgen05 kind::mxf4 -----------------------------------------------------------------------------------------
+// Operand without swizzle, rows of 16 bytes in groups of eight (128 bytes): the layout of a piece of scales.
+__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (8ull << 16) | (8ull << 32) | (1ull << 46);
+}
+// 32 rows x 16 bytes to four columns of TMEM, the same for each of the four lane quarters
+template <int CG>
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+    if constexpr (CG == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// kind::mxf4: A = B = E2M1 (1 at bits 7 and 10), scales E8M0 (bit 23), K-major, M = m, N = n, K = 64. `id` is the byte
+// (0 or 2) of the 32-bit scale cells that holds the first of the two scales of a row.
+__device__ __forceinline__ uint32_t instr_desc_mxf4(int m, int n, uint32_t id) {
+    return (id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27) | (id << 29);
+}
+template <int CG>
+__device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+
+// ---- cluster ----------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t mx_cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void mx_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t mx_map_to_rank(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+// Default (CTA-scope) semantics: nothing but the arrival itself has to be seen by the other CTA (its own operands are ordered by its barriers).
+__device__ __forceinline__ void mx_arrive_remote(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// The roles that issue copies and MMAs run as whole warps with one elected lane at the instructions themselves: control flow, addresses and
+// descriptors are then uniform for the compiler. (As code of one lane, every operand went through a conversion to a uniform register
+// and a stage of the products took 1440 clocks to issue, 222 for a wait that had nothing to wait for.)
+__device__ __forceinline__ int mx_uniform_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
+__device__ __forceinline__ bool mx_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// Bounded wait of a whole warp; false on all lanes once the CTA has given up.
+__device__ __forceinline__ bool mx_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, wait_or_abort_slow(bar, parity, abort_flag, status, code, kWaitLimitNs) && !*abort_flag);
+}
+
+__device__ __forceinline__ float silu_times(float g, float u) { return g / (1.f + expf(-g)) * u; }
+__device__ __forceinline__ float load_bias(const void* bias, int dtype, size_t i) {
+    if (dtype == B200Q_DT_F32) return static_cast<const float*>(bias)[i];
+    if (dtype == B200Q_DT_F16) return __half2float(static_cast<const __half*>(bias)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[i]);
+}
+__device__ __forceinline__ void store_y(void* y, int dtype, size_t i, float v) {
+    if (dtype == B200Q_DT_F32) static_cast<float*>(y)[i] = v;
+    else if (dtype == B200Q_DT_F16) static_cast<__half*>(y)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
+}
 #endif
 
 }  // namespace b200q

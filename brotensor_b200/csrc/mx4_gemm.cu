@@ -40,61 +40,6 @@ struct MxParams {
     uint32_t tmem_cols;
 };
 
-// ---- tcgen05 kind::mxf4 -----------------------------------------------------------------------------------------
-// Operand without swizzle, rows of 16 bytes in groups of eight (128 bytes): the layout of a piece of scales.
-__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (8ull << 16) | (8ull << 32) | (1ull << 46);
-}
-// 32 rows x 16 bytes to four columns of TMEM, the same for each of the four lane quarters
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-// kind::mxf4: A = B = E2M1 (1 at bits 7 and 10), scales E8M0 (bit 23), K-major, M = 128, N = n, K = 64. `id` is the byte
-// (0 or 2) of the 32-bit scale cells that holds the first of the two scales of a row.
-__device__ __forceinline__ uint32_t instr_desc_mxf4(int n, uint32_t id) {
-    return (id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | (1u << 27) | (id << 29);
-}
-__device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-}
-
-// ---- cluster ----------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t mx_cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void mx_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t mx_map_to_rank(uint32_t saddr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-
-__device__ __forceinline__ float silu_times(float g, float u) { return g / (1.f + expf(-g)) * u; }
-__device__ __forceinline__ float load_bias(const void* bias, int dtype, size_t i) {
-    if (dtype == B200Q_DT_F32) return static_cast<const float*>(bias)[i];
-    if (dtype == B200Q_DT_F16) return __half2float(static_cast<const __half*>(bias)[i]);
-    return __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[i]);
-}
-__device__ __forceinline__ void store_y(void* y, int dtype, size_t i, float v) {
-    if (dtype == B200Q_DT_F32) static_cast<float*>(y)[i] = v;
-    else if (dtype == B200Q_DT_F16) static_cast<__half*>(y)[i] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
-}
-
 template <int MATS>  // weight matrices: 1, or 2 for silu(gate) * up
 __global__ void __launch_bounds__(kMxThreads) mx4_gemm_kernel(const MxParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -104,7 +49,7 @@ __global__ void __launch_bounds__(kMxThreads) mx4_gemm_kernel(const MxParams p) 
     __shared__ int abort_flag;
     __shared__ int out_row[kMxTileRows];  // row of Y of each activation row of the tile
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = mx_uniform_warp(), lane = tid & 31;
     const uint32_t crank = p.split > 1 ? mx_cluster_rank() : 0u;
     const int64_t work = (int64_t)(blockIdx.x / (unsigned)p.split);
     const int64_t x_tile = work / p.row_tiles;
@@ -152,67 +97,68 @@ __global__ void __launch_bounds__(kMxThreads) mx4_gemm_kernel(const MxParams p) 
 
     const uint32_t sf_col0 = (uint32_t)(MATS * p.n_cols);  // scales behind the accumulators: per stage 8 columns for each matrix, 8 for X
     if (warp == 0) {
-        if (lane == 0) {
-            const uint8_t* w0 = p.W + (size_t)expert * p.w_expert_bytes + mx_tile_offset(row_tile, kt0, p.k_tiles);
-            const uint8_t* w1 = MATS == 2 ? p.W_up + (size_t)expert * p.w_expert_bytes + mx_tile_offset(row_tile, kt0, p.k_tiles) : nullptr;
-            const uint8_t* x = p.X + mx_tile_offset(x_tile, kt0, p.k_tiles);
-            const uint32_t x_bytes = (uint32_t)n_mma * 128u;
-            int slot = 0;
-            uint32_t phase = 1;
-            for (int kt = 0; kt < n_kt; ++kt) {
-                if (!wait_or_abort<true>(smem_u32(&bar_empty[slot]), phase, &abort_flag, p.status, kDevTimeoutEmpty)) break;
-                const uint32_t full = smem_u32(&bar_full[slot]), dst = sbase + slot * p.stage_bytes;
+        const uint8_t* w0 = p.W + (size_t)expert * p.w_expert_bytes + mx_tile_offset(row_tile, kt0, p.k_tiles);
+        const uint8_t* w1 = MATS == 2 ? p.W_up + (size_t)expert * p.w_expert_bytes + mx_tile_offset(row_tile, kt0, p.k_tiles) : nullptr;
+        const uint8_t* x = p.X + mx_tile_offset(x_tile, kt0, p.k_tiles);
+        const uint32_t x_bytes = (uint32_t)n_mma * 128u;
+        int slot = 0;
+        uint32_t phase = 1;
+        for (int kt = 0; kt < n_kt; ++kt) {
+            if (!mx_warp_wait(smem_u32(&bar_empty[slot]), phase, &abort_flag, p.status, kDevTimeoutEmpty)) break;
+            const uint32_t full = smem_u32(&bar_full[slot]), dst = sbase + slot * p.stage_bytes;
+            if (mx_elect()) {
                 mbar_arrive_expect_tx(full, MATS * kMxTileBytes + x_bytes + kMxSfBytes);
-                bulk_g2s(dst, w0 + (size_t)kt * kMxTileBytes, kMxTileBytes, full);
-                if (MATS == 2) bulk_g2s(dst + kMxTileBytes, w1 + (size_t)kt * kMxTileBytes, kMxTileBytes, full);
-                bulk_g2s(dst + MATS * kMxTileBytes + kMxSfBytes, x + (size_t)kt * kMxTileBytes, x_bytes, full);
-                bulk_g2s(dst + MATS * kMxTileBytes, x + (size_t)kt * kMxTileBytes + kMxQBytes, kMxSfBytes, full);
-                ++issued;
-                if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
+                bulk_g2s(dst, w0, kMxTileBytes, full);
+                if (MATS == 2) bulk_g2s(dst + kMxTileBytes, w1, kMxTileBytes, full);
+                bulk_g2s(dst + MATS * kMxTileBytes + kMxSfBytes, x, x_bytes, full);
+                bulk_g2s(dst + MATS * kMxTileBytes, x + kMxQBytes, kMxSfBytes, full);
             }
+            __syncwarp();
+            w0 += kMxTileBytes;
+            if (MATS == 2) w1 += kMxTileBytes;
+            x += kMxTileBytes;
+            ++issued;
+            if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
         }
-        __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            int slot = 0;
-            uint32_t phase = 0;
-            const uint32_t id0 = instr_desc_mxf4(n_mma, 0), id2 = instr_desc_mxf4(n_mma, 2);
-            for (int kt = 0; kt < n_kt; ++kt) {
-                if (!wait_or_abort<true>(smem_u32(&bar_full[slot]), phase, &abort_flag, p.status, kDevTimeoutFull)) break;
-                tc_fence_after();
-                const uint32_t st = sbase + slot * p.stage_bytes, xs = st + MATS * kMxTileBytes;
-                const uint32_t sf = tmem_base + sf_col0 + (uint32_t)(slot * 8 * (MATS + 1));
+        int slot = 0;
+        uint32_t phase = 0;
+        const uint32_t id0 = instr_desc_mxf4(kMxTileRows, n_mma, 0), id2 = instr_desc_mxf4(kMxTileRows, n_mma, 2);
+        for (int kt = 0; kt < n_kt; ++kt) {
+            if (!mx_warp_wait(smem_u32(&bar_full[slot]), phase, &abort_flag, p.status, kDevTimeoutFull)) break;
+            tc_fence_after();
+            const uint32_t st = sbase + slot * p.stage_bytes, xs = st + MATS * kMxTileBytes;
+            const uint32_t sf = tmem_base + sf_col0 + (uint32_t)(slot * 8 * (MATS + 1));
+            const int left = p.K - (kt0 + kt) * kMxTileK;  // columns beyond K are zeros: whole steps of them are left out
+            if (mx_elect()) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int m = 0; m < MATS; ++m) tmem_cp_scales(sf + 8 * m + 4 * h, smem_desc_scales(st + m * kMxTileBytes + kMxQBytes + 512 * h));
-                    tmem_cp_scales(sf + 8 * MATS + 4 * h, smem_desc_scales(xs + 512 * h));
+                    for (int m = 0; m < MATS; ++m) tmem_cp_scales<1>(sf + 8 * m + 4 * h, smem_desc_scales(st + m * kMxTileBytes + kMxQBytes + 512 * h));
+                    tmem_cp_scales<1>(sf + 8 * MATS + 4 * h, smem_desc_scales(xs + 512 * h));
                 }
-                const int left = p.K - (kt0 + kt) * kMxTileK;  // columns beyond K are zeros: whole steps of them are left out
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (64 * j < left) {
                         const uint64_t xd = smem_desc_sw128(xs + kMxSfBytes + 32 * j);
 #pragma unroll
                         for (int m = 0; m < MATS; ++m)
-                            umma_mxf4(tmem_base + m * p.n_cols, smem_desc_sw128(st + m * kMxTileBytes + 32 * j), xd, j & 1 ? id2 : id0,
-                                      sf + 8 * m + 4 * (j >> 1), sf + 8 * MATS + 4 * (j >> 1), (kt | j) != 0);
+                            umma_mxf4<1>(tmem_base + m * p.n_cols, smem_desc_sw128(st + m * kMxTileBytes + 32 * j), xd, j & 1 ? id2 : id0,
+                                         sf + 8 * m + 4 * (j >> 1), sf + 8 * MATS + 4 * (j >> 1), (kt | j) != 0);
                     }
                 }
                 umma_commit(smem_u32(&bar_empty[slot]));
-                if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
             }
-            if (rows > 0) umma_commit(smem_u32(&bar_accum));
+            __syncwarp();
+            if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
         }
+        if (rows > 0 && mx_elect()) umma_commit(smem_u32(&bar_accum));
         __syncwarp();
     }
     // ---- epilogue
     bool live = true;
     if (warp >= kMxEpilogueWarp0) {
-        if (rows > 0) {
-            const bool ok = gemm_wait(smem_u32(&bar_accum), 0, &abort_flag, p.status, kDevTimeoutMma);
-            live = __all_sync(0xffffffffu, ok && !*(volatile int*)&abort_flag);
-        }
+        if (rows > 0) live = mx_warp_wait(smem_u32(&bar_accum), 0, &abort_flag, p.status, kDevTimeoutMma);
         tc_fence_after();
         const int r = (warp & 3) * 32 + lane;  // weight row of the tile = TMEM lane
         const uint32_t tlane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
@@ -311,9 +257,19 @@ static int launch_mx_gemm(const MxParams& p, int64_t x_tiles, size_t smem, cudaS
     return B200Q_OK;
 }
 
+int launch_mx4_wide(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
+                    int E, int sms, int* status, cudaStream_t st);
+
+static int g_mx4_wide = 1;
+void mx4_set_wide(int v) { g_mx4_wide = v; }
+int mx4_get_wide() { return g_mx4_wide; }
+
 // One matrix (plan == nullptr: M rows of X) or the experts of a plan (buffer laid out for `pairs` pairs and E experts).
 int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K,
                     const int* plan, int64_t pairs, int E, int sms, int* status, cudaStream_t st) {
+    const bool many = plan ? pairs >= 64LL * E : M >= 192;
+    if (g_mx4_wide == 2 || (g_mx4_wide == 1 && many))
+        return launch_mx4_wide(W, W_up, X, bias, bias_dtype, Y, y_dtype, M, N, K, plan, pairs, E, sms, status, st);
     MxParams p = {};
     const int mats = W_up ? 2 : 1;
     p.W = static_cast<const uint8_t*>(W);

@@ -1,0 +1,384 @@
+// Products of MXFP4 images where there are many activation rows: the arithmetic of mx4_gemm.cu on tiles of 256 weight rows, activations
+// as the MMA's M, so that a thread of the epilogue holds one result row and stores 32 bytes of it at a time (weight rows as M, as the
+// small kernel has them, is 128 two-byte stores per thread and tile: 14 us of a 23 us tile at K = 4096).
+//
+// CG = 2: a pair of CTAs runs one tcgen05.mma.cta_group::2 of 256 activation rows x 256 weight rows; each CTA fetches its 128
+// activation rows and half of the weight rows (the scales of all 256), 35 KB per 256 columns and SM instead of 51 KB - the operand stream from the L2 is
+// what bounds these tiles, the tensor pipe would take 68 B a clock and SM. CG = 1: one CTA, 128 x 256, for groups of fewer rows.
+// The two halves of the weight rows are two row tiles of one matrix, or (GATED) the same row tile of gate and up: columns c and
+// 128 + c of the accumulator then meet in silu(gate) * up in the thread that holds both.
+//
+// Persistent CTAs; the ring runs on across tiles, so that the next tile's operands arrive while this one's results leave. 256 columns of TMEM are
+// the accumulator and 24 per stage hold scales, which leaves no room for a second accumulator: the eight epilogue warps take the whole tile
+// into registers first (128 values a thread), give the accumulator back and convert and store while the next tile runs.
+//   warp 0  loader    warp 1  TMEM, MMAs (the pair's leader)    warp 2  relay: this CTA's stage has landed -> leader
+//   warps 4..11  epilogue
+#include "mx4_common.cuh"
+
+namespace b200q {
+
+constexpr int kWideThreads = 384, kWideEpilogueWarp0 = 4, kWideMaxStages = 6;
+
+struct WideParams {
+    const uint8_t* W;      // image of the (gate) weights; expert e's lies e * w_expert_bytes behind
+    const uint8_t* W_up;
+    const uint8_t* X;
+    const void* bias;
+    void* Y;
+    int* status;
+    size_t w_expert_bytes;
+    const int4* tiles;     // grouped: {expert, first place, rows, tiles from here to the expert's end}; nullptr: one matrix
+    const int* n_tiles;
+    const int* order;
+    int M, N, K, k_tiles;
+    int row_tiles;         // 128-row tiles of a weight matrix
+    int w_tiles;           // 256-wide tiles of results: pairs of row tiles, or (gated) row tiles
+    int bias_dtype, y_dtype;
+    int n_stages;
+};
+
+template <int CG>
+__device__ __forceinline__ void wide_alloc(uint32_t slot) {
+    if constexpr (CG == 1) asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
+    else asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
+    if constexpr (CG == 1) asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    else asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+template <int CG>
+__device__ __forceinline__ void wide_dealloc(uint32_t base) {
+    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void wide_commit(uint32_t bar) {
+    if constexpr (CG == 1) {
+        umma_commit(bar);
+    } else {
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mx_map_to_rank(bar, 1)) : "memory");
+    }
+}
+
+// 16 neighbouring results of a row, `left` of them inside the matrix; `wide`: rows are multiples of 32 bytes and start on them
+template <typename T>
+__device__ __forceinline__ void store16(T* dst, const float (&v)[16], int left, bool wide) {
+    if (wide && left >= 16) {
+        constexpr int W = sizeof(T) == 4 ? 16 : 8;
+        uint32_t w[W];
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i]);
+        } else {
+            union {
+                T e[16];
+                uint32_t u[8];
+            } o;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o.e[i] = from_f32<T>(v[i]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = o.u[i];
+        }
+#pragma unroll
+        for (int i = 0; i < W; i += 8)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(dst) + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]),
+                         "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                         : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < left) dst[i] = from_f32<T>(v[i]);
+    }
+}
+
+template <int CG, bool GATED>
+__global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WideParams p) {
+    constexpr int kBTiles = CG == 1 ? 2 : 1;  // weight row tiles in this CTA's shared memory
+    constexpr int kStageBytes = kMxTileBytes + kBTiles * kMxQBytes + 2 * kMxSfBytes;
+    constexpr int kSfCols = 24;               // per stage: 8 columns of activations' scales, 16 of weights'
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    __shared__ uint64_t bar_full[kWideMaxStages];   // this CTA's stage has landed
+    __shared__ uint64_t bar_peer[kWideMaxStages];   // leader: the other CTA's stage has landed
+    __shared__ uint64_t bar_empty[kWideMaxStages];  // the MMAs on the stage have retired
+    __shared__ uint64_t bar_accum, bar_free;        // tile complete; leader: accumulator taken by all epilogue warps
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int abort_flag;
+
+    const int tid = threadIdx.x, warp = mx_uniform_warp(), lane = tid & 31;
+    const uint32_t crank = CG == 2 ? mx_cluster_rank() : 0u;
+    const int worker = (int)blockIdx.x / CG, workers = (int)gridDim.x / CG;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < p.n_stages; ++s) {
+            mbar_init(smem_u32(&bar_full[s]), 1);
+            mbar_init(smem_u32(&bar_peer[s]), 1);
+            mbar_init(smem_u32(&bar_empty[s]), 1);
+        }
+        mbar_init(smem_u32(&bar_accum), 1);
+        mbar_init(smem_u32(&bar_free), 8 * CG);
+        fence_mbar_init();
+    }
+    if (warp == 1) wide_alloc<CG>(smem_u32(&tmem_base_slot));
+    grid_dep_launch();
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2) mx_cluster_sync();
+    tc_fence_after();
+    grid_dep_wait();
+    const uint32_t tmem_base = tmem_base_slot;
+
+    // A unit is CG neighbouring activation tiles of one group; an item is a unit x a 256-wide tile of weights. The item's
+    // number says its unit and tile; in a grouped product units begin at tiles an even distance from their group's end or start (below).
+    const int x_tiles = p.tiles ? (int)ld_dep_u32(p.n_tiles) : (p.M + kMxTileRows - 1) / kMxTileRows;
+    const int units = (x_tiles + CG - 1) / CG;
+    const int items = units * p.w_tiles;
+    constexpr int kGroup = 8;  // units whose items are neighbours: the operands of concurrent tiles are shared in the L2
+    struct Item {
+        int x_tile, w_tile, rows, expert, first;
+    };
+    auto item_of = [&](int i, Item& it) {
+        int unit;
+        if (p.tiles) {
+            unit = i / p.w_tiles;
+            it.w_tile = i - unit * p.w_tiles;
+        } else {
+            const int per = kGroup * p.w_tiles, g = i / per, in = i - g * per, size = min(kGroup, units - g * kGroup);
+            it.w_tile = in / size;
+            unit = g * kGroup + in - it.w_tile * size;
+        }
+        it.x_tile = unit * CG + (int)crank;
+        it.expert = 0;
+        it.first = it.x_tile * kMxTileRows;
+        if (p.tiles) {
+            const uint4 t = ld_dep_u4(p.tiles + it.x_tile);
+            it.expert = (int)t.x;
+            it.first = (int)t.y;
+            it.rows = (int)t.z;
+        } else {
+            it.rows = max(min(kMxTileRows, p.M - it.first), 0);
+        }
+    };
+
+    int issued = 0;
+    if (warp == 0) {
+        int slot = 0;
+        uint32_t phase = 1;
+        bool ok = true;
+        for (int i = worker; ok && i < items; i += workers) {
+            Item it;
+            item_of(i, it);
+            // the last row tile of an odd number stands in for the one behind it, whose results are not stored
+            const int t0 = GATED ? it.w_tile : 2 * it.w_tile, t1 = GATED ? it.w_tile : min(2 * it.w_tile + 1, p.row_tiles - 1);
+            const uint8_t* w0 = p.W + (size_t)it.expert * p.w_expert_bytes + mx_tile_offset(t0, 0, p.k_tiles);
+            const uint8_t* w1 = (GATED ? p.W_up : p.W) + (size_t)it.expert * p.w_expert_bytes + mx_tile_offset(t1, 0, p.k_tiles);
+            const uint8_t* x = p.X + mx_tile_offset(it.x_tile, 0, p.k_tiles);
+            const uint32_t x_bytes = (uint32_t)((it.rows + 7) & ~7) * 128u;
+            // (a pair's second tile may lie behind the last: nothing of it is fetched, its rows of the accumulator are not used)
+            const uint32_t bytes = (x_bytes ? x_bytes + kMxSfBytes : 0u) + kBTiles * kMxQBytes + 2 * kMxSfBytes;
+            for (int kt = 0; kt < p.k_tiles; ++kt) {
+                if (!(ok = mx_warp_wait(smem_u32(&bar_empty[slot]), phase, &abort_flag, p.status, kDevTimeoutEmpty))) break;
+                const uint32_t full = smem_u32(&bar_full[slot]), dst = sbase + slot * kStageBytes, b = dst + kMxTileBytes;
+                if (mx_elect()) {
+                    mbar_arrive_expect_tx(full, bytes);
+                    if (x_bytes == kMxQBytes) {
+                        bulk_g2s(dst, x, kMxTileBytes, full);
+                    } else if (x_bytes) {
+                        bulk_g2s(dst, x, x_bytes, full);
+                        bulk_g2s(dst + kMxQBytes, x + kMxQBytes, kMxSfBytes, full);
+                    }
+                    // [activations and their scales][weights: tile(s)][scales of both tiles]
+                    if constexpr (CG == 1) {
+                        bulk_g2s(b, w0, kMxQBytes, full);
+                        bulk_g2s(b + kMxQBytes, w1, kMxQBytes, full);
+                    } else {
+                        bulk_g2s(b, crank ? w1 : w0, kMxQBytes, full);
+                    }
+                    bulk_g2s(b + kBTiles * kMxQBytes, w0 + kMxQBytes, kMxSfBytes, full);
+                    bulk_g2s(b + kBTiles * kMxQBytes + kMxSfBytes, w1 + kMxQBytes, kMxSfBytes, full);
+                }
+                __syncwarp();
+                x += kMxTileBytes;
+                w0 += kMxTileBytes;
+                w1 += kMxTileBytes;
+                ++issued;
+                if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
+            }
+        }
+    } else if (warp == 2) {
+        if (CG == 2 && crank == 1) {
+            int slot = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int i = worker; ok && i < items; i += workers)
+                for (int kt = 0; kt < p.k_tiles; ++kt) {
+                    if (!(ok = mx_warp_wait(smem_u32(&bar_full[slot]), phase, &abort_flag, p.status, kDevTimeoutFull))) break;
+                    if (mx_elect()) mx_arrive_remote(mx_map_to_rank(smem_u32(&bar_peer[slot]), 0));
+                    __syncwarp();
+                    if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
+                }
+        }
+    } else if (warp == 1) {
+        if (crank == 0) {
+            int slot = 0;
+            uint32_t phase = 0, free_phase = 1;
+            const uint32_t id0 = instr_desc_mxf4(128 * CG, 256, 0), id2 = instr_desc_mxf4(128 * CG, 256, 2);
+            bool ok = true;
+            for (int i = worker; ok && i < items; i += workers) {
+                if (!(ok = mx_warp_wait(smem_u32(&bar_free), free_phase, &abort_flag, p.status, kDevTimeoutEmpty))) break;
+                free_phase ^= 1;
+                for (int kt = 0; kt < p.k_tiles; ++kt) {
+                    if (!(ok = mx_warp_wait(smem_u32(&bar_full[slot]), phase, &abort_flag, p.status, kDevTimeoutFull))) break;
+                    if (CG == 2 && !(ok = mx_warp_wait(smem_u32(&bar_peer[slot]), phase, &abort_flag, p.status, kDevTimeoutFull))) break;
+                    tc_fence_after();
+                    const uint32_t a = sbase + slot * kStageBytes, b = a + kMxTileBytes, bs = b + kBTiles * kMxQBytes;
+                    const uint32_t sf = tmem_base + 256u + (uint32_t)(slot * kSfCols);
+                    const int left = p.K - kt * kMxTileK;
+                    if (mx_elect()) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            tmem_cp_scales<CG>(sf + 4 * h, smem_desc_scales(a + kMxQBytes + 512 * h));
+                            tmem_cp_scales<CG>(sf + 8 + 8 * h, smem_desc_scales(bs + 512 * h));
+                            tmem_cp_scales<CG>(sf + 12 + 8 * h, smem_desc_scales(bs + kMxSfBytes + 512 * h));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (64 * j < left)
+                                umma_mxf4<CG>(tmem_base, smem_desc_sw128(a + 32 * j), smem_desc_sw128(b + 32 * j), j & 1 ? id2 : id0, sf + 4 * (j >> 1), sf + 8 + 8 * (j >> 1), (kt | j) != 0);
+                        wide_commit<CG>(smem_u32(&bar_empty[slot]));
+                        if (kt + 1 == p.k_tiles) wide_commit<CG>(smem_u32(&bar_accum));
+                    }
+                    __syncwarp();
+                    if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
+                }
+            }
+        }
+    } else if (warp >= kWideEpilogueWarp0) {
+        const int half = (warp - kWideEpilogueWarp0) >> 2, r = (warp & 3) * 32 + lane;  // activation row of the tile = TMEM lane
+        const uint32_t tlane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t free_bar = CG == 2 ? mx_map_to_rank(smem_u32(&bar_free), 0) : smem_u32(&bar_free);
+        const size_t elem = p.y_dtype == B200Q_DT_F32 ? 4 : 2;
+        const bool wide = ((size_t)p.N * elem) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.Y) & 31) == 0;
+        uint32_t phase = 0;
+        for (int i = worker; i < items; i += workers) {
+            Item it;
+            item_of(i, it);
+            const int row = r < it.rows ? (p.tiles ? (int)ld_dep_u32(p.order + it.first + r) : it.first + r) : -1;
+            if (!mx_warp_wait(smem_u32(&bar_accum), phase, &abort_flag, p.status, kDevTimeoutMma)) break;
+            phase ^= 1;
+            tc_fence_after();
+            // plain: columns 128 half ..; gated: gate columns 64 half .. in acc[0..63], up columns behind them
+            uint32_t acc[8][16];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) tmem_ld16(tlane + (uint32_t)(GATED ? (c < 4 ? 64 * half + 16 * c : 128 + 64 * half + 16 * (c - 4)) : 128 * half + 16 * c), acc[c]);
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (CG == 2) mx_arrive_remote(free_bar);
+                else mbar_arrive(free_bar);
+            }
+            const int n0 = GATED ? it.w_tile * 128 + 64 * half : it.w_tile * 256 + 128 * half;
+            if (row >= 0) {
+#pragma unroll
+                for (int c = 0; c < (GATED ? 4 : 8); ++c) {
+                    const int n = n0 + 16 * c;
+                    if (n < p.N) {
+                        float v[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            v[j] = __uint_as_float(acc[c][j]);
+                            if constexpr (GATED) v[j] = silu_times(v[j], __uint_as_float(acc[4 + (c & 3)][j]));
+                        }
+                        if (!GATED && p.bias) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (n + j < p.N) v[j] += load_bias(p.bias, p.bias_dtype, (size_t)it.expert * p.N + n + j);
+                        }
+                        const size_t o = (size_t)row * p.N + n;
+                        if (p.y_dtype == B200Q_DT_F32) store16(static_cast<float*>(p.Y) + o, v, p.N - n, wide);
+                        else if (p.y_dtype == B200Q_DT_F16) store16(static_cast<__half*>(p.Y) + o, v, p.N - n, wide);
+                        else store16(static_cast<__nv_bfloat16*>(p.Y) + o, v, p.N - n, wide);
+                    }
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && abort_flag) {  // given up: let the copies in flight land before the CTA's shared memory is given away
+        for (int kt = max(issued - p.n_stages, 0); kt < issued; ++kt)
+            mbar_wait_bounded(smem_u32(&bar_full[kt % p.n_stages]), (uint32_t)(kt / p.n_stages) & 1u, p.status, kDevTimeoutFull, 1u << 12);
+    }
+    __syncwarp();
+    if (CG == 2) mx_cluster_sync();  // nobody leaves while the pair's MMAs or arrivals may still reach it
+    if (warp == 1) wide_dealloc<CG>(tmem_base);
+}
+
+template <int CG, bool GATED>
+static int launch_wide(const WideParams& q, int64_t x_tiles, int sms, cudaStream_t st) {
+    auto kern = mx4_wide_kernel<CG, GATED>;
+    static bool configured[64] = {};
+    int dev = 0;
+    B200Q_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        B200Q_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    WideParams p = q;
+    constexpr int stage = kMxTileBytes + (CG == 1 ? 2 : 1) * kMxQBytes + 2 * kMxSfBytes;
+    p.n_stages = (220 * 1024) / stage;
+    if (p.n_stages > kWideMaxStages) p.n_stages = kWideMaxStages;
+    const int64_t items = (x_tiles + CG - 1) / CG * p.w_tiles;
+    if (items > (1LL << 30)) return fail(B200Q_ERR_UNSUPPORTED, "mx4: %lld tiles are more than one launch takes", (long long)items);
+    int workers = sms / CG;
+    if (items < workers) workers = (int)items;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(workers * CG));
+    cfg.blockDim = dim3(kWideThreads);
+    cfg.dynamicSmemBytes = (size_t)p.n_stages * stage + 1024;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_option() >= 0 ? 2 : 1;
+    B200Q_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
+    return B200Q_OK;
+}
+
+int launch_mx4_wide(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
+                    int E, int sms, int* status, cudaStream_t st) {
+    WideParams p = {};
+    p.W = static_cast<const uint8_t*>(W);
+    p.W_up = static_cast<const uint8_t*>(W_up);
+    p.X = static_cast<const uint8_t*>(X);
+    p.bias = bias;
+    p.bias_dtype = bias_dtype;
+    p.Y = Y;
+    p.y_dtype = y_dtype;
+    p.status = status;
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    p.k_tiles = mx_k_tiles(K);
+    p.row_tiles = (int)mx_row_tiles(N);
+    p.w_tiles = W_up ? p.row_tiles : (p.row_tiles + 1) / 2;
+    int64_t x_tiles = mx_row_tiles(M);
+    if (plan) {
+        const MoePlanLayout l = moe_plan_layout(pairs, E);
+        p.w_expert_bytes = mx_image_bytes(N, K);
+        p.tiles = reinterpret_cast<const int4*>(plan + l.tiles);
+        p.n_tiles = plan + l.n_tiles;
+        p.order = plan + l.order;
+        x_tiles = l.max_tiles;
+        return W_up ? launch_wide<1, true>(p, x_tiles, sms, st) : launch_wide<1, false>(p, x_tiles, sms, st);
+    }
+    return W_up ? launch_wide<2, true>(p, x_tiles, sms, st) : launch_wide<2, false>(p, x_tiles, sms, st);
+}
+
+}  // namespace b200q

@@ -371,6 +371,8 @@ int b200q_device_status(int* status_out);
  *   "gemv_i8"     Q8_0 / Q4_K, 2..8 activation rows, K = 2048 / 4096: 1 = the integer tensor-core kernel where it is
  *                 the faster one (default), 2 = for every such call, 0 = never
  *   "gemv_lean"   0 = never take the trimmed instantiation of the integer-dot kernel (FP32 in and out, no bias)
+ *   "mx4_wide"    products of MXFP4 images: 1 (default) = the kernel of 256-wide tiles where there are many activation rows, 2 = for
+ *                 every call, 0 = never
  *   "wait_limit_us" bound of the decode kernels' device-side waits (stage barriers, peer arrival) in
  *                 microseconds; 0 = one second. Tests shorten it to see a wait run out.
  *   "last_kernel" (read only) the kernel of the calling thread's last linear call, its last pass: 1 plain-load GEMV, 2 warp-MMA

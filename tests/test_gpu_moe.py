@@ -5,7 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import mx4_reference as ref
-from test_gpu_mx4 import BF16, F16, F32, _check, _randn, _weights
+from test_gpu_mx4 import BF16, F16, F32, _check, _randn, _weights, route  # noqa: F401
 
 from brotensor_b200 import ops
 
@@ -97,7 +97,7 @@ def _products(Ws, x, ids, N, bias=None):
 
 @pytest.mark.parametrize("per_pair", [False, True])
 @pytest.mark.parametrize("T,k,E,N,K", [(1, 1, 1, 32, 32), (1, 8, 128, 256, 512), (3, 2, 8, 77, 96), (50, 4, 16, 200, 544), (300, 2, 3, 130, 256), (96, 6, 64, 384, 1408), (700, 4, 5, 128, 320)])
-def test_experts(T, k, E, N, K, per_pair):
+def test_experts(T, k, E, N, K, per_pair, route):
     W, w = _weights(N, K, N + K, count=E)
     ids = _ids(T, k, E, T) if k <= E else torch.zeros(T, k, dtype=torch.int32)
     x = _randn((T, k, K) if per_pair else (T, K), BF16, 3)
@@ -110,7 +110,7 @@ def test_experts(T, k, E, N, K, per_pair):
 
 @pytest.mark.parametrize("x_dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("y_dtype", [F32, F16, BF16])
-def test_experts_bias_types_and_pairs_without_an_expert(x_dtype, y_dtype):
+def test_experts_bias_types_and_pairs_without_an_expert(x_dtype, y_dtype, route):
     T, k, E, N, K = 40, 3, 6, 150, 288
     W, w = _weights(N, K, 5, count=E)
     ids = _ids(T, k, E, 6, drop=0.25)
@@ -127,7 +127,7 @@ def test_experts_bias_types_and_pairs_without_an_expert(x_dtype, y_dtype):
 
 
 @pytest.mark.parametrize("T,k,E,N,K", [(1, 8, 32, 768, 2048), (2, 2, 4, 40, 96), (200, 4, 6, 300, 512), (900, 2, 4, 128, 288)])
-def test_swiglu(T, k, E, N, K):
+def test_swiglu(T, k, E, N, K, route):
     (G, g), (U, u) = _weights(N, K, 11, count=E), _weights(N, K, 12, count=E)
     ids = _ids(T, k, E, 13)
     x = _randn((T, K), F16, 14)

@@ -90,9 +90,17 @@ def test_pack_takes_blocks_from_any_byte():
     assert torch.equal(ops.mx4_dequantize(ops.mx4_pack(shifted[5:], 64, 256), 64, 256), ref.matrix(b, 64, 256).float())
 
 
+@pytest.fixture(params=[0, 1, 2], ids=["small tiles", "as routed", "wide tiles"])
+def route(request):
+    """Both kernels take every call; each is held to the definition whatever the routing rule says."""
+    ops.set_option("mx4_wide", request.param)
+    yield
+    ops.set_option("mx4_wide", 1)
+
+
 @pytest.mark.parametrize("M", [1, 2, 16, 17, 100, 128, 129, 300])
 @pytest.mark.parametrize("N,K", [(128, 256), (1, 32), (77, 96), (200, 544), (384, 1024)])
-def test_linear(M, N, K):
+def test_linear(M, N, K, route):
     W, w = _weights(N, K, N + K)
     x = _randn((M, K), F32, M + K)
     q = ref.quantise(x)
@@ -103,7 +111,7 @@ def test_linear(M, N, K):
 @pytest.mark.parametrize("x_dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("y_dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("bias", [False, True])
-def test_linear_types(x_dtype, y_dtype, bias):
+def test_linear_types(x_dtype, y_dtype, bias, route):
     M, N, K = 21, 150, 416
     W, w = _weights(N, K, 7)
     x = _randn((M, K), x_dtype, 8)
@@ -113,8 +121,8 @@ def test_linear_types(x_dtype, y_dtype, bias):
     _check(ops.mx4_linear(W, x, N, bias=b, out_dtype=y_dtype), want, q.abs() @ w[0].abs().T, K, b.double() if bias else None)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (8, 1024, 14336), (45, 2560, 6912), (513, 640, 4096), (1, 128, 65536), (2, 130, 2304 + 32)])
-def test_linear_long(M, N, K):
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (8, 1024, 14336), (45, 2560, 6912), (513, 640, 4096), (1, 128, 65536), (2, 130, 2304 + 32), (2100, 5000, 512)])
+def test_linear_long(M, N, K, route):
     W, w = _weights(N, K, 17)
     x = _randn((M, K), BF16, 18)
     q = ref.quantise(x)
