@@ -7,7 +7,7 @@ namespace b200q {
 int device_facts(int* sms, int** status);  // api.cu
 int launch_mx4_quantise(const void* x, int x_dtype, int64_t rows, int K, void* image, const int* place, int copies, int sms, cudaStream_t st);
 int launch_mx4_dequantise(const void* image, int64_t rows, int K, void* out, int out_dtype, int sms, cudaStream_t st);
-int launch_mx4_pack(const void* blocks, int64_t rows, int64_t count, int K, void* image, int sms, cudaStream_t st);
+int launch_mx4_pack(const void* blocks, int64_t rows, int64_t count, int K, void* image, cudaStream_t st);
 int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K,
                     const int* plan, int64_t pairs, int E, int sms, int* status, cudaStream_t st);
 int launch_moe_topk(const void* logits, int dtype, int64_t tokens, int E, int k, int normalize, float scale, int* ids, float* weights, int sms, cudaStream_t st);
@@ -47,7 +47,7 @@ int b200q_mx4_pack(const void* blocks, int64_t count, int64_t rows, int K, void*
     if (!on(image, 16)) return fail(B200Q_ERR_BAD_ARG, "mx4_pack: the image must be 16-byte aligned");
     int sms, *status;
     if (int rc = device_facts(&sms, &status)) return rc;
-    return launch_mx4_pack(blocks, rows, count, K, image, sms, static_cast<cudaStream_t>(stream));
+    return launch_mx4_pack(blocks, rows, count, K, image, static_cast<cudaStream_t>(stream));
 }
 
 int b200q_mx4_quantize(const void* x, int x_dtype, int64_t rows, int K, void* image, void* stream) {

@@ -107,28 +107,30 @@ __global__ void __launch_bounds__(kPlanBlockPairs) moe_count_kernel(const int* i
 }
 
 // pass 2, one block, thread e is expert e: hist becomes the first place of each block's pairs; offsets and tiles
-__global__ void __launch_bounds__(kMaxExperts) moe_scan_kernel(int E, int blocks, int* hist, int* offsets, int* n_tiles, int4* tiles) {
-    __shared__ int warp_pairs[32], warp_tiles[32];
+__global__ void __launch_bounds__(kMaxExperts) moe_scan_kernel(int E, int blocks, int* hist, int* offsets, int* n_tiles, int4* tiles, int4* units) {
+    __shared__ int warp_pairs[32], warp_tiles[32], warp_units[32];
     grid_dep_launch();
     grid_dep_wait();
     const int e = threadIdx.x, lane = e & 31, warp = e >> 5;
     int total = 0;
     if (e < E)
         for (int b = 0; b < blocks; ++b) total += (int)ld_dep_u32(hist + (int64_t)b * E + e);
-    const int my_tiles = (total + kMxTileRows - 1) / kMxTileRows;
-    int pairs_to = total, tiles_to = my_tiles;  // inclusive sums
+    const int my_tiles = (total + kMxTileRows - 1) / kMxTileRows, my_units = (my_tiles + 1) / 2;
+    int pairs_to = total, tiles_to = my_tiles, units_to = my_units;  // inclusive sums
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, pairs_to, o), c = __shfl_up_sync(0xffffffffu, tiles_to, o);
-        if (lane >= o) { pairs_to += a; tiles_to += c; }
+        const int a = __shfl_up_sync(0xffffffffu, pairs_to, o), c = __shfl_up_sync(0xffffffffu, tiles_to, o), d = __shfl_up_sync(0xffffffffu, units_to, o);
+        if (lane >= o) { pairs_to += a; tiles_to += c; units_to += d; }
     }
-    if (lane == 31) { warp_pairs[warp] = pairs_to; warp_tiles[warp] = tiles_to; }
+    if (lane == 31) { warp_pairs[warp] = pairs_to; warp_tiles[warp] = tiles_to; warp_units[warp] = units_to; }
     __syncthreads();
-    for (int w = 0; w < warp; ++w) { pairs_to += warp_pairs[w]; tiles_to += warp_tiles[w]; }
+    for (int w = 0; w < warp; ++w) { pairs_to += warp_pairs[w]; tiles_to += warp_tiles[w]; units_to += warp_units[w]; }
     if (e < E) {
         int at = pairs_to - total;
         offsets[e] = at;
         for (int i = 0; i < my_tiles; ++i) tiles[tiles_to - my_tiles + i] = make_int4(e, at + i * kMxTileRows, min(kMxTileRows, total - i * kMxTileRows), 0);
+        for (int i = 0; i < my_units; ++i)
+            units[units_to - my_units + i] = make_int4(e, at + i * 2 * kMxTileRows, min(2 * kMxTileRows, total - i * 2 * kMxTileRows), tiles_to - my_tiles + 2 * i);
         for (int b = 0; b < blocks; ++b) {
             int* h = hist + (int64_t)b * E + e;
             const int c = (int)ld_dep_u32(h);
@@ -138,7 +140,8 @@ __global__ void __launch_bounds__(kMaxExperts) moe_scan_kernel(int E, int blocks
     }
     if (e == kMaxExperts - 1) {
         offsets[E] = pairs_to;
-        *n_tiles = tiles_to;
+        n_tiles[0] = tiles_to;
+        n_tiles[1] = units_to;
     }
 }
 
@@ -254,11 +257,11 @@ int launch_moe_topk(const void* logits, int dtype, int64_t tokens, int E, int k,
 int launch_moe_plan(const int* ids, int64_t pairs, int E, int* plan, cudaStream_t st) {
     const MoePlanLayout l = moe_plan_layout(pairs, E);
     int *offsets = plan, *order = plan + l.order, *place = plan + l.place, *n_tiles = plan + l.n_tiles, *hist = plan + l.hist;
-    int4* tiles = reinterpret_cast<int4*>(plan + l.tiles);
+    int4 *tiles = reinterpret_cast<int4*>(plan + l.tiles), *units = reinterpret_cast<int4*>(plan + l.units);
     const bool dep = pdl_option() >= 0;
     const dim3 grid((unsigned)l.hist_blocks), block(kPlanBlockPairs);
     if (l.hist_blocks) B200Q_CUDA_TRY(launch_dep(dep, moe_count_kernel, grid, block, (size_t)E * 4, st, ids, pairs, E, hist));
-    B200Q_CUDA_TRY(launch_dep(dep, moe_scan_kernel, dim3(1), dim3(kMaxExperts), 0, st, E, l.hist_blocks, hist, offsets, n_tiles, tiles));
+    B200Q_CUDA_TRY(launch_dep(dep, moe_scan_kernel, dim3(1), dim3(kMaxExperts), 0, st, E, l.hist_blocks, hist, offsets, n_tiles, tiles, units));
     if (l.hist_blocks) {
         const size_t smem = (size_t)64 * E;
         static bool configured[64] = {};

@@ -56,134 +56,200 @@ __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], uint32_t& sca
     return out;
 }
 
+// Blocks of the three kernels cover a patch of rows x column tiles: of a block's eight warps 2^wide stand side by side along a row, the others
+// on the rows below, and each takes `kBatch` neighbouring column tiles, whose loads are in flight together. No index needs a division (with
+// one number per 256 columns, divided into row and column, the kernels ran at a quarter of the memory's rate).
+struct Patch {
+    int64_t row;
+    int kt;
+    __device__ __forceinline__ Patch(int wide, int batch) {
+        const int warp = threadIdx.x >> 5;
+        row = ((int64_t)blockIdx.x << (3 - wide)) + (warp >> wide);
+        kt = (((int)blockIdx.y << wide) + (warp & ((1 << wide) - 1))) * batch;
+    }
+};
+
 // A warp quantises 256 columns of a row: lane 4 b + s elements 8 s .. 8 s + 7 of block b. The row's 128 bytes of the image are
 // one line. With `place`, row i of x is written to the rows place[i * copies + c], c < copies, of the image (-1: not).
-template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) mx4_quantise_kernel(const T* x, int64_t rows, int K, int k_tiles, uint8_t* image, const int* place, int copies) {
-    grid_dep_launch();
+// Dependents are let go once the predecessor has finished: what they read beside this kernel's results is then in place.
+template <typename T, int kBatch>
+__global__ void __launch_bounds__(kQuantThreads) mx4_quantise_kernel(const T* x, int64_t rows, int K, int k_tiles, int wide, uint8_t* image, const int* place, int copies) {
     grid_dep_wait();
+    grid_dep_launch();
     const int lane = threadIdx.x & 31, b = lane >> 2, s = lane & 3;
-    const int64_t items = rows * k_tiles, warps = (int64_t)gridDim.x * (kQuantThreads / 32);
-    constexpr int kBatch = 4;  // items whose loads are in flight together
-    for (int64_t i0 = (int64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); i0 < items; i0 += warps * kBatch) {
-        float v[kBatch][8];
+    const Patch at(wide, kBatch);
+    if (at.row >= rows || at.kt >= k_tiles) return;
+    const T* src = x + at.row * K + (int64_t)at.kt * kMxTileK + 8 * lane;
+    float v[kBatch][8];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
+        if ((at.kt + u) * kMxTileK + 8 * lane < K) load8(src + u * kMxTileK, v[u]);
+    }
+    uint32_t q[kBatch], word[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        uint32_t sc;
+        q[u] = quantise8(v[u], sc);
+        // the four scales of the lane's half (blocks 0..3 or 4..7) in one word
+        word[u] = sc << (8 * (b & 3));
+        word[u] |= __shfl_xor_sync(0xffffffffu, word[u], 4);
+        word[u] |= __shfl_xor_sync(0xffffffffu, word[u], 8);
+    }
+    for (int c = 0; c < copies; ++c) {
+        const int64_t to = place ? (int64_t)(int)ld_dep_u32(place + at.row * copies + c) : at.row;
+        if (to < 0) continue;
+        const int r = (int)(to & 127);
+        uint8_t* tile = image + mx_tile_offset(to >> 7, at.kt, k_tiles);
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const int64_t i = i0 + u * warps, row = i / k_tiles;
-            const int k = (int)(i - row * k_tiles) * kMxTileK + 8 * lane;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
-            if (i < items && k < K) load8(x + row * K + k, v[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const int64_t i = i0 + u * warps;
-            if (i >= items) break;
-            const int64_t row = i / k_tiles;
-            const int kt = (int)(i - row * k_tiles);
-            uint32_t sc;
-            const uint32_t q = quantise8(v[u], sc);
-            // the four scales of the lane's half (blocks 0..3 or 4..7) in one word
-            uint32_t word = sc << (8 * (b & 3));
-            word |= __shfl_xor_sync(0xffffffffu, word, 4);
-            word |= __shfl_xor_sync(0xffffffffu, word, 8);
-            for (int c = 0; c < (place ? copies : 1); ++c) {
-                const int64_t to = place ? (int64_t)(int)ld_dep_u32(place + row * copies + c) : row;
-                if (to < 0) continue;
-                uint8_t* tile = image + mx_tile_offset(to >> 7, kt, k_tiles);
-                const int r = (int)(to & 127);
-                *reinterpret_cast<uint32_t*>(tile + mx_chunk_offset(r, b) + 4 * s) = q;
-                if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_offset(r, lane >> 4)) = word;
+            if (at.kt + u < k_tiles) {
+                *reinterpret_cast<uint32_t*>(tile + u * kMxTileBytes + mx_chunk_offset(r, b) + 4 * s) = q[u];
+                if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + u * kMxTileBytes + mx_scale_offset(r, lane >> 4)) = word[u];
             }
         }
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) mx4_dequantise_kernel(const uint8_t* image, int64_t rows, int K, int k_tiles, T* out) {
+template <typename T, int kBatch>
+__global__ void __launch_bounds__(kQuantThreads) mx4_dequantise_kernel(const uint8_t* image, int64_t rows, int K, int k_tiles, int wide, T* out) {
     grid_dep_launch();
     grid_dep_wait();
     const int lane = threadIdx.x & 31, b = lane >> 2, s = lane & 3;
-    const int64_t items = rows * k_tiles, warps = (int64_t)gridDim.x * (kQuantThreads / 32);
-    for (int64_t i = (int64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); i < items; i += warps) {
-        const int64_t row = i / k_tiles;
-        const int kt = (int)(i - row * k_tiles), k = kt * kMxTileK + 8 * lane, r = (int)(row & 127);
-        if (k >= K) continue;
-        const uint8_t* tile = image + mx_tile_offset(row >> 7, kt, k_tiles);
-        const uint32_t q = ld_dep_u32(tile + mx_chunk_offset(r, b) + 4 * s);
-        const float d = e8m0_to_f32(ld_dep_u32(tile + mx_scale_offset(r, b >> 2)) >> (8 * (b & 3)) & 255u);
+    const Patch at(wide, kBatch);
+    if (at.row >= rows || at.kt >= k_tiles) return;
+    const int r = (int)(at.row & 127);
+    const uint8_t* tile = image + mx_tile_offset(at.row >> 7, at.kt, k_tiles);
+    uint32_t q[kBatch], word[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        q[u] = word[u] = 0u;
+        if (at.kt + u < k_tiles) {
+            q[u] = ld_dep_u32(tile + u * kMxTileBytes + mx_chunk_offset(r, b) + 4 * s);
+            word[u] = ld_dep_u32(tile + u * kMxTileBytes + mx_scale_offset(r, b >> 2));
+        }
+    }
+    T* dst = out + at.row * K + (int64_t)at.kt * kMxTileK + 8 * lane;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        if ((at.kt + u) * kMxTileK + 8 * lane >= K) continue;
+        const float d = e8m0_to_f32(word[u] >> (8 * (b & 3)) & 255u);
         union {
             T e[8];
             uint4 v[sizeof(T) / 2];
         } o;
+        uint32_t h[4];  // pairs of values in FP16, which holds them exactly
+        asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+            "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+            : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+            : "r"(q[u]));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o.e[j] = from_f32<T>(e2m1_to_f32(q >> (4 * j) & 15u) * d);
-        uint4* dst = reinterpret_cast<uint4*>(out + row * K + k);
+        for (int j = 0; j < 8; ++j) o.e[j] = from_f32<T>(h2f(j & 1 ? h[j >> 1] >> 16 : h[j >> 1] & 0xFFFFu) * d);
+        uint4* to = reinterpret_cast<uint4*>(dst + u * kMxTileK);
+        if (sizeof(T) == 4 && (reinterpret_cast<uintptr_t>(out) & 31) == 0) {  // whole sectors; two 16-byte stores leave halves
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(o.v[0].x), "r"(o.v[0].y), "r"(o.v[0].z), "r"(o.v[0].w), "r"(o.v[sizeof(T) / 2 - 1].x),
+                         "r"(o.v[sizeof(T) / 2 - 1].y), "r"(o.v[sizeof(T) / 2 - 1].z), "r"(o.v[sizeof(T) / 2 - 1].w)
+                         : "memory");
+        } else {
 #pragma unroll
-        for (int j = 0; j < (int)(sizeof(T) / 2); ++j) dst[j] = o.v[j];
+            for (int j = 0; j < (int)(sizeof(T) / 2); ++j) to[j] = o.v[j];
+        }
     }
 }
 
 // A file's blocks -> image. A warp moves 256 columns of a row: lane 4 b + s makes elements 8 s .. 8 s + 7 of block b, which are
 // low (s < 2) or high nibbles of eight neighbouring bytes. `rows` of each of `count` matrices, each with an image of its own.
-__global__ void __launch_bounds__(kQuantThreads) mx4_pack_kernel(const uint8_t* blocks, int64_t rows, int64_t count, int K, int k_tiles, uint8_t* image) {
+__global__ void __launch_bounds__(kQuantThreads) mx4_pack_kernel(const uint8_t* blocks, int64_t rows, int64_t count, int K, int k_tiles, int wide, uint8_t* image) {
     grid_dep_launch();
     grid_dep_wait();
     const int lane = threadIdx.x & 31, b = lane >> 2, s = lane & 3;
-    const int64_t items = count * rows * k_tiles, warps = (int64_t)gridDim.x * (kQuantThreads / 32);
-    const size_t bytes = mx_image_bytes(rows, K);
-    for (int64_t i = (int64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); i < items; i += warps) {
-        const int64_t at = i / k_tiles, mat = at / rows, row = at - mat * rows;
-        const int kt = (int)(i - at * k_tiles), r = (int)(row & 127);
-        uint32_t q = 0, sc = 0;
-        if (kt * kMxTileK + 32 * b < K) {
-            const uint8_t* blk = blocks + ((size_t)at * (K / 32) + (size_t)kt * 8 + b) * kMxBlockBytes;
-            sc = blk[0];
+    const Patch at(wide, 1);
+    if (at.row >= rows * count || at.kt >= k_tiles) return;
+    const int64_t mat = at.row / rows, row = at.row - mat * rows;
+    const int r = (int)(row & 127);
+    uint32_t q = 0, sc = 0;
+    if (at.kt * kMxTileK + 32 * b < K) {
+        const uint8_t* blk = blocks + ((size_t)at.row * (K / 32) + (size_t)at.kt * 8 + b) * kMxBlockBytes;
+        sc = blk[0];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) q |= ((uint32_t)blk[1 + 8 * (s & 1) + j] >> (s & 2 ? 4 : 0) & 15u) << (4 * j);
-        }
-        uint32_t word = sc << (8 * (b & 3));
-        word |= __shfl_xor_sync(0xffffffffu, word, 4);
-        word |= __shfl_xor_sync(0xffffffffu, word, 8);
-        uint8_t* tile = image + (size_t)mat * bytes + mx_tile_offset(row >> 7, kt, k_tiles);
-        *reinterpret_cast<uint32_t*>(tile + mx_chunk_offset(r, b) + 4 * s) = q;
-        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_offset(r, lane >> 4)) = word;
+        for (int j = 0; j < 8; ++j) q |= ((uint32_t)blk[1 + 8 * (s & 1) + j] >> (s & 2 ? 4 : 0) & 15u) << (4 * j);
     }
+    uint32_t word = sc << (8 * (b & 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    uint8_t* tile = image + (size_t)mat * mx_image_bytes(rows, K) + mx_tile_offset(row >> 7, at.kt, k_tiles);
+    *reinterpret_cast<uint32_t*>(tile + mx_chunk_offset(r, b) + 4 * s) = q;
+    if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_offset(r, lane >> 4)) = word;
 }
 
-static unsigned quant_grid(int64_t items, int batch, int sms) {
-    const int64_t blocks = (items + (int64_t)batch * (kQuantThreads / 32) - 1) / (batch * (kQuantThreads / 32)), most = (int64_t)sms * 8;
-    return (unsigned)(blocks < most ? blocks : most);
+// Warps side by side (2^wide of a block's eight) until a block's rows are all there are; blocks along the rows, and along the columns.
+struct PatchGrid {
+    dim3 grid;
+    int wide;
+    bool ok;
+    PatchGrid(int64_t rows, int k_tiles, int batch) {
+        const int64_t along = (k_tiles + batch - 1) / batch;
+        wide = 0;
+        while (wide < 3 && (2 << wide) <= along && rows <= (int64_t)4 >> wide) ++wide;
+        const int64_t x = (rows + (8 >> wide) - 1) >> (3 - wide), y = (along + (1 << wide) - 1) >> wide;
+        ok = x <= 2147483647LL && y <= 65535;
+        grid = dim3((unsigned)x, (unsigned)y);
+    }
+};
+
+template <typename T, int kBatch>
+static int quantise_typed(const void* x, int64_t rows, int K, void* image, const int* place, int copies, cudaStream_t st) {
+    const int kt = mx_k_tiles(K);
+    const PatchGrid g(rows, kt, kBatch);
+    if (!g.ok) return fail(B200Q_ERR_UNSUPPORTED, "mx4_quantize: %lld x %d is more than one launch takes", (long long)rows, K);
+    B200Q_CUDA_TRY(launch_dep(pdl_option() >= 0, mx4_quantise_kernel<T, kBatch>, g.grid, dim3(kQuantThreads), 0, st, static_cast<const T*>(x), rows, K, kt, g.wide,
+                              static_cast<uint8_t*>(image), place, copies));
+    return B200Q_OK;
 }
+template <typename T, int kBatch>
+static int dequantise_typed(const void* image, int64_t rows, int K, void* out, cudaStream_t st) {
+    const int kt = mx_k_tiles(K);
+    const PatchGrid g(rows, kt, kBatch);
+    if (!g.ok) return fail(B200Q_ERR_UNSUPPORTED, "mx4_dequantize: %lld x %d is more than one launch takes", (long long)rows, K);
+    B200Q_CUDA_TRY(launch_dep(pdl_option() >= 0, mx4_dequantise_kernel<T, kBatch>, g.grid, dim3(kQuantThreads), 0, st, static_cast<const uint8_t*>(image), rows, K, kt, g.wide,
+                              static_cast<T*>(out)));
+    return B200Q_OK;
+}
+
+// Several column tiles a warp once every SM has 32 warps' worth of single ones: four of 16-bit elements, two of FP32, measured on 14336 x 4096 BF16
+// and 2000 x 4096 FP32 (two, four, eight: 31.9, 27.3, 28.8 us and 6.5, 6.8, 7.6; back 26.5, 24.9, 26.8 and, with 16-byte stores, 10.4, 11.8, 15.7).
+template <typename T>
+constexpr int kBatchOf = sizeof(T) == 4 ? 2 : 4;
 
 int launch_mx4_quantise(const void* x, int x_dtype, int64_t rows, int K, void* image, const int* place, int copies, int sms, cudaStream_t st) {
-    const int kt = mx_k_tiles(K);
-    const int64_t items = rows * kt;
-    // few items: one each per warp, so that they spread over the SMs
-    const dim3 grid(quant_grid(items, items > (int64_t)sms * 32 ? 4 : 1, sms)), block(kQuantThreads);
-    const bool dep = pdl_option() >= 0;
-    uint8_t* im = static_cast<uint8_t*>(image);
-    if (x_dtype == B200Q_DT_F32) B200Q_CUDA_TRY(launch_dep(dep, mx4_quantise_kernel<float>, grid, block, 0, st, static_cast<const float*>(x), rows, K, kt, im, place, copies));
-    else if (x_dtype == B200Q_DT_F16) B200Q_CUDA_TRY(launch_dep(dep, mx4_quantise_kernel<__half>, grid, block, 0, st, static_cast<const __half*>(x), rows, K, kt, im, place, copies));
-    else B200Q_CUDA_TRY(launch_dep(dep, mx4_quantise_kernel<__nv_bfloat16>, grid, block, 0, st, static_cast<const __nv_bfloat16*>(x), rows, K, kt, im, place, copies));
-    return B200Q_OK;
+    const bool many = rows * mx_k_tiles(K) > (int64_t)sms * 32;
+    auto run = [&](auto zero) {
+        using T = decltype(zero);
+        return many ? quantise_typed<T, kBatchOf<T>>(x, rows, K, image, place, copies, st) : quantise_typed<T, 1>(x, rows, K, image, place, copies, st);
+    };
+    return x_dtype == B200Q_DT_F32 ? run(0.f) : x_dtype == B200Q_DT_F16 ? run(__half()) : run(__nv_bfloat16());
 }
 
 int launch_mx4_dequantise(const void* image, int64_t rows, int K, void* out, int out_dtype, int sms, cudaStream_t st) {
-    const int kt = mx_k_tiles(K);
-    const dim3 grid(quant_grid(rows * kt, 1, sms)), block(kQuantThreads);
-    const bool dep = pdl_option() >= 0;
-    const uint8_t* im = static_cast<const uint8_t*>(image);
-    if (out_dtype == B200Q_DT_F32) B200Q_CUDA_TRY(launch_dep(dep, mx4_dequantise_kernel<float>, grid, block, 0, st, im, rows, K, kt, static_cast<float*>(out)));
-    else if (out_dtype == B200Q_DT_F16) B200Q_CUDA_TRY(launch_dep(dep, mx4_dequantise_kernel<__half>, grid, block, 0, st, im, rows, K, kt, static_cast<__half*>(out)));
-    else B200Q_CUDA_TRY(launch_dep(dep, mx4_dequantise_kernel<__nv_bfloat16>, grid, block, 0, st, im, rows, K, kt, static_cast<__nv_bfloat16*>(out)));
-    return B200Q_OK;
+    const bool many = rows * mx_k_tiles(K) > (int64_t)sms * 32;
+    auto run = [&](auto zero) {
+        using T = decltype(zero);
+        return many ? dequantise_typed<T, kBatchOf<T>>(image, rows, K, out, st) : dequantise_typed<T, 1>(image, rows, K, out, st);
+    };
+    return out_dtype == B200Q_DT_F32 ? run(0.f) : out_dtype == B200Q_DT_F16 ? run(__half()) : run(__nv_bfloat16());
 }
 
-int launch_mx4_pack(const void* blocks, int64_t rows, int64_t count, int K, void* image, int sms, cudaStream_t st) {
+int launch_mx4_pack(const void* blocks, int64_t rows, int64_t count, int K, void* image, cudaStream_t st) {
     const int kt = mx_k_tiles(K);
-    const dim3 grid(quant_grid(count * rows * kt, 1, sms)), block(kQuantThreads);
-    B200Q_CUDA_TRY(launch_dep(pdl_option() >= 0, mx4_pack_kernel, grid, block, 0, st, static_cast<const uint8_t*>(blocks), rows, count, K, kt, static_cast<uint8_t*>(image)));
+    const PatchGrid g(rows * count, kt, 1);
+    if (!g.ok) return fail(B200Q_ERR_UNSUPPORTED, "mx4_pack: %lld x %lld x %d is more than one launch takes", (long long)count, (long long)rows, K);
+    B200Q_CUDA_TRY(launch_dep(pdl_option() >= 0, mx4_pack_kernel, g.grid, dim3(kQuantThreads), 0, st, static_cast<const uint8_t*>(blocks), rows, count, K, kt, g.wide,
+                              static_cast<uint8_t*>(image)));
     return B200Q_OK;
 }
 

@@ -2,9 +2,9 @@
 // as the MMA's M, so that a thread of the epilogue holds one result row and stores 32 bytes of it at a time (weight rows as M, as the
 // small kernel has them, is 128 two-byte stores per thread and tile: 14 us of a 23 us tile at K = 4096).
 //
-// CG = 2: a pair of CTAs runs one tcgen05.mma.cta_group::2 of 256 activation rows x 256 weight rows; each CTA fetches its 128
-// activation rows and half of the weight rows (the scales of all 256), 35 KB per 256 columns and SM instead of 51 KB - the operand stream from the L2 is
-// what bounds these tiles, the tensor pipe would take 68 B a clock and SM. CG = 1: one CTA, 128 x 256, for groups of fewer rows.
+// A pair of CTAs runs one tcgen05.mma.cta_group::2 of 256 activation rows x 256 weight rows; each CTA fetches its 128
+// activation rows and half of the weight rows (the scales of all 256), 35 KB per 256 columns and SM. One CTA on 128 x 256 would fetch 51 KB for the
+// same work per SM, and the operand stream from the L2 (about 12 TB/s) is what bounds these tiles.
 // The two halves of the weight rows are two row tiles of one matrix, or (GATED) the same row tile of gate and up: columns c and
 // 128 + c of the accumulator then meet in silu(gate) * up in the thread that holds both.
 //
@@ -17,7 +17,11 @@
 
 namespace b200q {
 
-constexpr int kWideThreads = 384, kWideEpilogueWarp0 = 4, kWideMaxStages = 6;
+constexpr int kWideThreads = 384, kWideEpilogueWarp0 = 4, kWideStages = 6;
+// [activations and their scales][half of the weight rows][scales of all weight rows]
+constexpr int kWideStageBytes = kMxTileBytes + kMxQBytes + 2 * kMxSfBytes;
+constexpr int kWideSfCols = 24;  // per stage: 8 TMEM columns of activations' scales, 16 of weights'
+
 
 struct WideParams {
     const uint8_t* W;      // image of the (gate) weights; expert e's lies e * w_expert_bytes behind
@@ -27,36 +31,24 @@ struct WideParams {
     void* Y;
     int* status;
     size_t w_expert_bytes;
-    const int4* tiles;     // grouped: {expert, first place, rows, tiles from here to the expert's end}; nullptr: one matrix
-    const int* n_tiles;
+    const int4* units;     // grouped: {expert, first place, rows, first tile} of two neighbouring tiles; nullptr: one matrix
+    const int* n_units;
     const int* order;
     int M, N, K, k_tiles;
     int row_tiles;         // 128-row tiles of a weight matrix
     int w_tiles;           // 256-wide tiles of results: pairs of row tiles, or (gated) row tiles
     int bias_dtype, y_dtype;
-    int n_stages;
 };
 
-template <int CG>
 __device__ __forceinline__ void wide_alloc(uint32_t slot) {
-    if constexpr (CG == 1) asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
-    else asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
-    if constexpr (CG == 1) asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    else asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
-template <int CG>
-__device__ __forceinline__ void wide_dealloc(uint32_t base) {
-    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
-    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory");
-}
-template <int CG>
+__device__ __forceinline__ void wide_dealloc(uint32_t base) { asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(base) : "memory"); }
+// arrives on the barrier in both CTAs once all MMAs issued so far have retired
 __device__ __forceinline__ void wide_commit(uint32_t bar) {
-    if constexpr (CG == 1) {
-        umma_commit(bar);
-    } else {
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mx_map_to_rank(bar, 1)) : "memory");
-    }
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mx_map_to_rank(bar, 1)) : "memory");
 }
 
 // 16 neighbouring results of a row, `left` of them inside the matrix; `wide`: rows are multiples of 32 bytes and start on them
@@ -90,47 +82,40 @@ __device__ __forceinline__ void store16(T* dst, const float (&v)[16], int left, 
     }
 }
 
-template <int CG, bool GATED>
+template <bool GATED>
 __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WideParams p) {
-    constexpr int kBTiles = CG == 1 ? 2 : 1;  // weight row tiles in this CTA's shared memory
-    constexpr int kStageBytes = kMxTileBytes + kBTiles * kMxQBytes + 2 * kMxSfBytes;
-    constexpr int kSfCols = 24;               // per stage: 8 columns of activations' scales, 16 of weights'
     extern __shared__ uint8_t smem_raw[];
     const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    __shared__ uint64_t bar_full[kWideMaxStages];   // this CTA's stage has landed
-    __shared__ uint64_t bar_peer[kWideMaxStages];   // leader: the other CTA's stage has landed
-    __shared__ uint64_t bar_empty[kWideMaxStages];  // the MMAs on the stage have retired
+    __shared__ uint64_t bar_full[kWideStages];   // this CTA's stage has landed; leader: and the other CTA's
+    __shared__ uint64_t bar_empty[kWideStages];  // the MMAs on the stage have retired
     __shared__ uint64_t bar_accum, bar_free;        // tile complete; leader: accumulator taken by all epilogue warps
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
 
     const int tid = threadIdx.x, warp = mx_uniform_warp(), lane = tid & 31;
-    const uint32_t crank = CG == 2 ? mx_cluster_rank() : 0u;
-    const int worker = (int)blockIdx.x / CG, workers = (int)gridDim.x / CG;
+    const uint32_t crank = mx_cluster_rank();
+    const int worker = (int)blockIdx.x / 2, workers = (int)gridDim.x / 2;
     if (tid == 0) {
         abort_flag = 0;
-        for (int s = 0; s < p.n_stages; ++s) {
-            mbar_init(smem_u32(&bar_full[s]), 1);
-            mbar_init(smem_u32(&bar_peer[s]), 1);
+        for (int s = 0; s < kWideStages; ++s) {
+            mbar_init(smem_u32(&bar_full[s]), crank == 0 ? 2 : 1);
             mbar_init(smem_u32(&bar_empty[s]), 1);
         }
         mbar_init(smem_u32(&bar_accum), 1);
-        mbar_init(smem_u32(&bar_free), 8 * CG);
+        mbar_init(smem_u32(&bar_free), 16);
         fence_mbar_init();
     }
-    if (warp == 1) wide_alloc<CG>(smem_u32(&tmem_base_slot));
+    if (warp == 1) wide_alloc(smem_u32(&tmem_base_slot));
     grid_dep_launch();
     tc_fence_before();
     __syncthreads();
-    if (CG == 2) mx_cluster_sync();
+    mx_cluster_sync();
     tc_fence_after();
     grid_dep_wait();
     const uint32_t tmem_base = tmem_base_slot;
 
-    // A unit is CG neighbouring activation tiles of one group; an item is a unit x a 256-wide tile of weights. The item's
-    // number says its unit and tile; in a grouped product units begin at tiles an even distance from their group's end or start (below).
-    const int x_tiles = p.tiles ? (int)ld_dep_u32(p.n_tiles) : (p.M + kMxTileRows - 1) / kMxTileRows;
-    const int units = (x_tiles + CG - 1) / CG;
+    // A unit is two neighbouring activation tiles of one group (or its last one); an item is a unit x a 256-wide tile of weights.
+    const int units = p.units ? (int)ld_dep_u32(p.n_units) : (p.M + 2 * kMxTileRows - 1) / (2 * kMxTileRows);
     const int items = units * p.w_tiles;
     constexpr int kGroup = 8;  // units whose items are neighbours: the operands of concurrent tiles are shared in the L2
     struct Item {
@@ -138,7 +123,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
     };
     auto item_of = [&](int i, Item& it) {
         int unit;
-        if (p.tiles) {
+        if (p.units) {
             unit = i / p.w_tiles;
             it.w_tile = i - unit * p.w_tiles;
         } else {
@@ -146,17 +131,18 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
             it.w_tile = in / size;
             unit = g * kGroup + in - it.w_tile * size;
         }
-        it.x_tile = unit * CG + (int)crank;
+        it.x_tile = unit * 2 + (int)crank;
         it.expert = 0;
         it.first = it.x_tile * kMxTileRows;
-        if (p.tiles) {
-            const uint4 t = ld_dep_u4(p.tiles + it.x_tile);
-            it.expert = (int)t.x;
-            it.first = (int)t.y;
-            it.rows = (int)t.z;
-        } else {
-            it.rows = max(min(kMxTileRows, p.M - it.first), 0);
+        it.rows = p.M - it.first;
+        if (p.units) {
+            const uint4 u = ld_dep_u4(p.units + unit);
+            it.expert = (int)u.x;
+            it.first = (int)u.y + (int)crank * kMxTileRows;
+            it.rows = (int)u.z - (int)crank * kMxTileRows;
+            it.x_tile = (int)u.w + (int)crank;
         }
+        it.rows = max(min(kMxTileRows, it.rows), 0);
     };
 
     int issued = 0;
@@ -174,10 +160,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
             const uint8_t* x = p.X + mx_tile_offset(it.x_tile, 0, p.k_tiles);
             const uint32_t x_bytes = (uint32_t)((it.rows + 7) & ~7) * 128u;
             // (a pair's second tile may lie behind the last: nothing of it is fetched, its rows of the accumulator are not used)
-            const uint32_t bytes = (x_bytes ? x_bytes + kMxSfBytes : 0u) + kBTiles * kMxQBytes + 2 * kMxSfBytes;
+            const uint32_t bytes = (x_bytes ? x_bytes + kMxSfBytes : 0u) + kMxQBytes + 2 * kMxSfBytes;
             for (int kt = 0; kt < p.k_tiles; ++kt) {
                 if (!(ok = mx_warp_wait(smem_u32(&bar_empty[slot]), phase, &abort_flag, p.status, kDevTimeoutEmpty))) break;
-                const uint32_t full = smem_u32(&bar_full[slot]), dst = sbase + slot * kStageBytes, b = dst + kMxTileBytes;
+                const uint32_t full = smem_u32(&bar_full[slot]), dst = sbase + slot * kWideStageBytes, b = dst + kMxTileBytes;
                 if (mx_elect()) {
                     mbar_arrive_expect_tx(full, bytes);
                     if (x_bytes == kMxQBytes) {
@@ -186,83 +172,76 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
                         bulk_g2s(dst, x, x_bytes, full);
                         bulk_g2s(dst + kMxQBytes, x + kMxQBytes, kMxSfBytes, full);
                     }
-                    // [activations and their scales][weights: tile(s)][scales of both tiles]
-                    if constexpr (CG == 1) {
-                        bulk_g2s(b, w0, kMxQBytes, full);
-                        bulk_g2s(b + kMxQBytes, w1, kMxQBytes, full);
-                    } else {
-                        bulk_g2s(b, crank ? w1 : w0, kMxQBytes, full);
-                    }
-                    bulk_g2s(b + kBTiles * kMxQBytes, w0 + kMxQBytes, kMxSfBytes, full);
-                    bulk_g2s(b + kBTiles * kMxQBytes + kMxSfBytes, w1 + kMxQBytes, kMxSfBytes, full);
+                    bulk_g2s(b, crank ? w1 : w0, kMxQBytes, full);
+                    bulk_g2s(b + kMxQBytes, w0 + kMxQBytes, kMxSfBytes, full);
+                    bulk_g2s(b + kMxQBytes + kMxSfBytes, w1 + kMxQBytes, kMxSfBytes, full);
                 }
                 __syncwarp();
                 x += kMxTileBytes;
                 w0 += kMxTileBytes;
                 w1 += kMxTileBytes;
                 ++issued;
-                if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
+                if (++slot == kWideStages) { slot = 0; phase ^= 1; }
             }
         }
     } else if (warp == 2) {
-        if (CG == 2 && crank == 1) {
+        if (crank == 1) {
             int slot = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (int i = worker; ok && i < items; i += workers)
                 for (int kt = 0; kt < p.k_tiles; ++kt) {
                     if (!(ok = mx_warp_wait(smem_u32(&bar_full[slot]), phase, &abort_flag, p.status, kDevTimeoutFull))) break;
-                    if (mx_elect()) mx_arrive_remote(mx_map_to_rank(smem_u32(&bar_peer[slot]), 0));
+                    if (mx_elect()) mx_arrive_remote(mx_map_to_rank(smem_u32(&bar_full[slot]), 0));
                     __syncwarp();
-                    if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
+                    if (++slot == kWideStages) { slot = 0; phase ^= 1; }
                 }
         }
     } else if (warp == 1) {
         if (crank == 0) {
             int slot = 0;
             uint32_t phase = 0, free_phase = 1;
-            const uint32_t id0 = instr_desc_mxf4(128 * CG, 256, 0), id2 = instr_desc_mxf4(128 * CG, 256, 2);
+            const uint32_t id0 = instr_desc_mxf4(256, 256, 0), id2 = instr_desc_mxf4(256, 256, 2);
             bool ok = true;
             for (int i = worker; ok && i < items; i += workers) {
                 if (!(ok = mx_warp_wait(smem_u32(&bar_free), free_phase, &abort_flag, p.status, kDevTimeoutEmpty))) break;
                 free_phase ^= 1;
                 for (int kt = 0; kt < p.k_tiles; ++kt) {
                     if (!(ok = mx_warp_wait(smem_u32(&bar_full[slot]), phase, &abort_flag, p.status, kDevTimeoutFull))) break;
-                    if (CG == 2 && !(ok = mx_warp_wait(smem_u32(&bar_peer[slot]), phase, &abort_flag, p.status, kDevTimeoutFull))) break;
                     tc_fence_after();
-                    const uint32_t a = sbase + slot * kStageBytes, b = a + kMxTileBytes, bs = b + kBTiles * kMxQBytes;
-                    const uint32_t sf = tmem_base + 256u + (uint32_t)(slot * kSfCols);
+                    const uint32_t a = sbase + slot * kWideStageBytes, b = a + kMxTileBytes, bs = b + kMxQBytes;
+                    const uint32_t sf = tmem_base + 256u + (uint32_t)(slot * kWideSfCols);
                     const int left = p.K - kt * kMxTileK;
                     if (mx_elect()) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            tmem_cp_scales<CG>(sf + 4 * h, smem_desc_scales(a + kMxQBytes + 512 * h));
-                            tmem_cp_scales<CG>(sf + 8 + 8 * h, smem_desc_scales(bs + 512 * h));
-                            tmem_cp_scales<CG>(sf + 12 + 8 * h, smem_desc_scales(bs + kMxSfBytes + 512 * h));
+                            tmem_cp_scales<2>(sf + 4 * h, smem_desc_scales(a + kMxQBytes + 512 * h));
+                            tmem_cp_scales<2>(sf + 8 + 8 * h, smem_desc_scales(bs + 512 * h));
+                            tmem_cp_scales<2>(sf + 12 + 8 * h, smem_desc_scales(bs + kMxSfBytes + 512 * h));
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
                             if (64 * j < left)
-                                umma_mxf4<CG>(tmem_base, smem_desc_sw128(a + 32 * j), smem_desc_sw128(b + 32 * j), j & 1 ? id2 : id0, sf + 4 * (j >> 1), sf + 8 + 8 * (j >> 1), (kt | j) != 0);
-                        wide_commit<CG>(smem_u32(&bar_empty[slot]));
-                        if (kt + 1 == p.k_tiles) wide_commit<CG>(smem_u32(&bar_accum));
+                                umma_mxf4<2>(tmem_base, smem_desc_sw128(a + 32 * j), smem_desc_sw128(b + 32 * j), j & 1 ? id2 : id0, sf + 4 * (j >> 1), sf + 8 + 8 * (j >> 1), (kt | j) != 0);
+                        wide_commit(smem_u32(&bar_empty[slot]));
+                        if (kt + 1 == p.k_tiles) wide_commit(smem_u32(&bar_accum));
                     }
                     __syncwarp();
-                    if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
+                    if (++slot == kWideStages) { slot = 0; phase ^= 1; }
                 }
             }
         }
     } else if (warp >= kWideEpilogueWarp0) {
         const int half = (warp - kWideEpilogueWarp0) >> 2, r = (warp & 3) * 32 + lane;  // activation row of the tile = TMEM lane
         const uint32_t tlane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t free_bar = CG == 2 ? mx_map_to_rank(smem_u32(&bar_free), 0) : smem_u32(&bar_free);
+        const uint32_t free_bar = mx_map_to_rank(smem_u32(&bar_free), 0);
         const size_t elem = p.y_dtype == B200Q_DT_F32 ? 4 : 2;
         const bool wide = ((size_t)p.N * elem) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.Y) & 31) == 0;
         uint32_t phase = 0;
         for (int i = worker; i < items; i += workers) {
             Item it;
             item_of(i, it);
-            const int row = r < it.rows ? (p.tiles ? (int)ld_dep_u32(p.order + it.first + r) : it.first + r) : -1;
+            const int row = r < it.rows ? (p.units ? (int)ld_dep_u32(p.order + it.first + r) : it.first + r) : -1;
             if (!mx_warp_wait(smem_u32(&bar_accum), phase, &abort_flag, p.status, kDevTimeoutMma)) break;
             phase ^= 1;
             tc_fence_after();
@@ -273,10 +252,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
             tmem_ld_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-                if (CG == 2) mx_arrive_remote(free_bar);
-                else mbar_arrive(free_bar);
-            }
+            if (lane == 0) mx_arrive_remote(free_bar);
             const int n0 = GATED ? it.w_tile * 128 + 64 * half : it.w_tile * 256 + 128 * half;
             if (row >= 0) {
 #pragma unroll
@@ -307,40 +283,36 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && abort_flag) {  // given up: let the copies in flight land before the CTA's shared memory is given away
-        for (int kt = max(issued - p.n_stages, 0); kt < issued; ++kt)
-            mbar_wait_bounded(smem_u32(&bar_full[kt % p.n_stages]), (uint32_t)(kt / p.n_stages) & 1u, p.status, kDevTimeoutFull, 1u << 12);
+        for (int kt = max(issued - kWideStages, 0); kt < issued; ++kt)
+            mbar_wait_bounded(smem_u32(&bar_full[kt % kWideStages]), (uint32_t)(kt / kWideStages) & 1u, p.status, kDevTimeoutFull, 1u << 12);
     }
     __syncwarp();
-    if (CG == 2) mx_cluster_sync();  // nobody leaves while the pair's MMAs or arrivals may still reach it
-    if (warp == 1) wide_dealloc<CG>(tmem_base);
+    mx_cluster_sync();  // nobody leaves while the pair's MMAs or arrivals may still reach it
+    if (warp == 1) wide_dealloc(tmem_base);
 }
 
-template <int CG, bool GATED>
-static int launch_wide(const WideParams& q, int64_t x_tiles, int sms, cudaStream_t st) {
-    auto kern = mx4_wide_kernel<CG, GATED>;
+template <bool GATED>
+static int launch_wide(const WideParams& p, int64_t units, int sms, cudaStream_t st) {
+    auto kern = mx4_wide_kernel<GATED>;
+    constexpr int smem = kWideStages * kWideStageBytes + 1024;
     static bool configured[64] = {};
     int dev = 0;
     B200Q_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        B200Q_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024));
+        B200Q_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    WideParams p = q;
-    constexpr int stage = kMxTileBytes + (CG == 1 ? 2 : 1) * kMxQBytes + 2 * kMxSfBytes;
-    p.n_stages = (220 * 1024) / stage;
-    if (p.n_stages > kWideMaxStages) p.n_stages = kWideMaxStages;
-    const int64_t items = (x_tiles + CG - 1) / CG * p.w_tiles;
+    const int64_t items = units * p.w_tiles;
     if (items > (1LL << 30)) return fail(B200Q_ERR_UNSUPPORTED, "mx4: %lld tiles are more than one launch takes", (long long)items);
-    int workers = sms / CG;
-    if (items < workers) workers = (int)items;
+    const int workers = items < sms / 2 ? (int)items : sms / 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(workers * CG));
+    cfg.gridDim = dim3((unsigned)(workers * 2));
     cfg.blockDim = dim3(kWideThreads);
-    cfg.dynamicSmemBytes = (size_t)p.n_stages * stage + 1024;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -351,6 +323,7 @@ static int launch_wide(const WideParams& q, int64_t x_tiles, int sms, cudaStream
     return B200Q_OK;
 }
 
+// One matrix (plan == nullptr: M rows of X) or the experts of a plan (buffer laid out for `pairs` pairs and E experts).
 int launch_mx4_wide(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
                     int E, int sms, int* status, cudaStream_t st) {
     WideParams p = {};
@@ -368,17 +341,16 @@ int launch_mx4_wide(const void* W, const void* W_up, const void* X, const void* 
     p.k_tiles = mx_k_tiles(K);
     p.row_tiles = (int)mx_row_tiles(N);
     p.w_tiles = W_up ? p.row_tiles : (p.row_tiles + 1) / 2;
-    int64_t x_tiles = mx_row_tiles(M);
+    int64_t units = (mx_row_tiles(M) + 1) / 2;
     if (plan) {
         const MoePlanLayout l = moe_plan_layout(pairs, E);
         p.w_expert_bytes = mx_image_bytes(N, K);
-        p.tiles = reinterpret_cast<const int4*>(plan + l.tiles);
-        p.n_tiles = plan + l.n_tiles;
+        p.units = reinterpret_cast<const int4*>(plan + l.units);
+        p.n_units = plan + l.n_tiles + 1;
         p.order = plan + l.order;
-        x_tiles = l.max_tiles;
-        return W_up ? launch_wide<1, true>(p, x_tiles, sms, st) : launch_wide<1, false>(p, x_tiles, sms, st);
+        units = l.max_units;
     }
-    return W_up ? launch_wide<2, true>(p, x_tiles, sms, st) : launch_wide<2, false>(p, x_tiles, sms, st);
+    return W_up ? launch_wide<true>(p, units, sms, st) : launch_wide<false>(p, units, sms, st);
 }
 
 }  // namespace b200q
