@@ -54,6 +54,9 @@ int launch_gemm_mm(int fmt, const void* W, const void* X, int x_dtype, const voi
 void mm_set_enabled(int v);
 void mx4_set_wide(int v);
 int mx4_get_wide();
+void mx4_set_few(int v);
+int mx4_get_few();
+void few_set(int, int);
 int mm_get_enabled();
 int mb_get_enabled();
 void i8_set_enabled(int v);
@@ -635,6 +638,8 @@ int b200q_set_option(const char* key, int value) {
     else if (!strcmp(key, "gemv_hm")) hm_set_enabled(value);
     else if (!strcmp(key, "gemm_mm")) mm_set_enabled(value);
     else if (!strcmp(key, "mx4_wide")) mx4_set_wide(value);
+    else if (!strcmp(key, "mx4_few")) mx4_set_few(value);
+    else if (!strcmp(key, "few_probe")) few_set(value & 15, value >> 4);
     else if (!strcmp(key, "gemv_step_fill")) dp_set_step_fill(value);
     else return fail(B200Q_ERR_BAD_ARG, "set_option: unknown key '%s'", key);
     return B200Q_OK;
@@ -654,6 +659,7 @@ int b200q_get_option(const char* key, int* out) {
     else if (!strcmp(key, "gemv_hm")) *out = hm_get_enabled();
     else if (!strcmp(key, "gemm_mm")) *out = mm_get_enabled();
     else if (!strcmp(key, "mx4_wide")) *out = mx4_get_wide();
+    else if (!strcmp(key, "mx4_few")) *out = mx4_get_few();
     else if (!strcmp(key, "gemv_tile_pairs")) *out = dp_get_tile_pairs();
     else if (!strcmp(key, "gemm_pair")) *out = gemm_get_pair();
     else if (!strcmp(key, "gemm_split")) *out = gemm_get_split();

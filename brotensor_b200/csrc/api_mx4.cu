@@ -10,6 +10,9 @@ int launch_mx4_dequantise(const void* image, int64_t rows, int K, void* out, int
 int launch_mx4_pack(const void* blocks, int64_t rows, int64_t count, int K, void* image, cudaStream_t st);
 int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K,
                     const int* plan, int64_t pairs, int E, int sms, int* status, cudaStream_t st);
+int launch_mx4_few(const void* W, const void* W_up, const void* X, int x_dtype, const void* bias, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
+                   int pairs_per_row, int E, int sms, int* status, cudaStream_t st, bool* taken);
+int mx4_get_few();
 int launch_moe_topk(const void* logits, int dtype, int64_t tokens, int E, int k, int normalize, float scale, int* ids, float* weights, int sms, cudaStream_t st);
 int launch_moe_plan(const int* ids, int64_t pairs, int E, int* plan, cudaStream_t st);
 int launch_moe_combine(const void* y, int dtype, const int* ids, const float* weights, int64_t tokens, int k, int N, int E, void* out, int sms, cudaStream_t st);
@@ -109,6 +112,16 @@ int b200q_mx4_linear(const void* W, const void* X, int x_dtype, const void* bias
     if (!on(X, 16)) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: X must be 16-byte aligned");
     if (!W || !Y) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: null pointer");
     if (int rc = check_ws("mx4_linear", ws, ws_bytes, b200q_mx4_linear_workspace_bytes(M, K))) return rc;
+    if (!on(W, 16)) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: images must be 16-byte aligned");
+    if (!on(Y, dtype_size(y_dtype))) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: Y is not aligned to its element size");
+    if (bias && !on(bias, dtype_size(x_dtype))) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: the bias is not aligned to its element size");
+    if (M <= mx4_get_few()) {
+        int sms, *status;
+        if (int rc = device_facts(&sms, &status)) return rc;
+        bool taken;
+        if (int rc = launch_mx4_few(W, nullptr, X, x_dtype, bias, Y, y_dtype, M, N, K, nullptr, 0, 1, 0, sms, status, static_cast<cudaStream_t>(stream), &taken)) return rc;
+        if (taken) return B200Q_OK;
+    }
     if (int rc = b200q_mx4_quantize(X, x_dtype, M, K, ws, stream)) return rc;
     return gemm_common("mx4_linear", W, ws, bias, x_dtype, Y, y_dtype, M, N, K, stream);
 }
@@ -164,6 +177,11 @@ static int experts_common(const char* op, const void* W, const void* W_up, const
     if (int rc = device_facts(&sms, &status)) return rc;
     const int64_t pairs = tokens * k;
     const int* pl = static_cast<const int*>(plan);
+    if (pairs <= mx4_get_few()) {
+        bool taken;
+        if (int rc = launch_mx4_few(W, W_up, X, x_dtype, bias, Y, y_dtype, 0, N, K, pl, pairs, x_per_pair ? 1 : k, E, sms, status, static_cast<cudaStream_t>(stream), &taken)) return rc;
+        if (taken) return B200Q_OK;
+    }
     const int* place = pl + moe_plan_layout(pairs, E).place;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (int rc = launch_mx4_quantise(X, x_dtype, x_per_pair ? pairs : tokens, K, ws, place, x_per_pair ? 1 : k, sms, st)) return rc;

@@ -54,6 +54,14 @@ inline __host__ MoePlanLayout moe_plan_layout(int64_t pairs, int E) {
     return l;
 }
 
+// Shared memory that a kernel with `cols` TMEM columns asks for, its own need being `bytes`: at least 456 bytes a column with the 2 KB of
+// static and reserved memory, so that CTAs which an SM takes by its 228 KB always find their columns too, whichever of these kernels
+// share it. (A CTA that waits for columns while its cluster's others hold theirs could otherwise wait for a CTA that waits for it.)
+inline size_t mx_smem_for_tmem(size_t bytes, uint32_t cols) {
+    const size_t least = (size_t)cols * 456 - 2048;
+    return bytes < least ? least : bytes;
+}
+
 #ifdef __CUDACC__
 __device__ __forceinline__ float e8m0_to_f32(uint32_t e) {  // 2^(e - 127); 0 is 2^-127, a subnormal
     return e == 255u ? __uint_as_float(0x7FC00000u) : e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23);
@@ -61,6 +69,55 @@ __device__ __forceinline__ float e8m0_to_f32(uint32_t e) {  // 2^(e - 127); 0 is
 __device__ __forceinline__ size_t mx_tile_offset(int64_t row_tile, int k_tile, int k_tiles) { return ((size_t)row_tile * k_tiles + k_tile) * kMxTileBytes; }
 __device__ __forceinline__ uint32_t mx_chunk_offset(int r, int b) { return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((b ^ (r & 7)) << 4)); }
 __device__ __forceinline__ uint32_t mx_scale_offset(int r, int half) { return (uint32_t)(kMxQBytes + half * 512 + (r & 31) * 16 + (r >> 5) * 4); }
+// Quantisation (OCP Microscaling Formats specification 1.0, 6.3): a block's exponent is floor(log2(largest magnitude)) - 2, which puts
+// the largest magnitude into [4, 8); elements are divided by that power of two - exact in FP32 - and rounded to the nearest E2M1
+// value, ties to the even one, magnitudes beyond 6 to 6. A block with an infinity or a NaN becomes NaN as a whole (e = 255), one of zeros e = 0.
+// Eight neighbouring elements in FP32.
+template <typename T>
+__device__ __forceinline__ void mx_load8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = ld_dep_f4(p), b = ld_dep_f4(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        union {
+            uint4 q;
+            T e[8];
+        } u;
+        u.q = ld_dep_u4(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(u.e[i]);
+    }
+}
+
+// A quad of lanes holds a block, eight elements each: returns the lane's eight nibbles and the block's scale byte.
+__device__ __forceinline__ uint32_t mx_quantise8(const float (&v)[8], uint32_t& scale) {
+    uint32_t top = 0;  // magnitudes as bits compare like magnitudes, infinities and NaNs above all
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int be = (int)(top >> 23);  // 0: a zero or a subnormal, below 2^-126 - the smallest scale serves
+    if (be == 255) {
+        scale = 255u;
+        return 0u;
+    }
+    const int e = max(be - 2, 0);  // biased exponent of the scale
+    scale = (uint32_t)e;
+    // 1 / scale = 2^(127 - e), 127 - e in -125 .. 127
+    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+    uint32_t out;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(out)
+        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
+    return out;
+}
+
 // ---- tcgen05 kind::mxf4 -----------------------------------------------------------------------------------------
 // Operand without swizzle, rows of 16 bytes in groups of eight (128 bytes): the layout of a piece of scales.
 __device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
@@ -111,6 +168,14 @@ __device__ __forceinline__ uint32_t mx_map_to_rank(uint32_t saddr, uint32_t rank
 }
 // Default (CTA-scope) semantics: nothing but the arrival itself has to be seen by the other CTA (its own operands are ordered by its barriers).
 __device__ __forceinline__ void mx_arrive_remote(uint32_t cluster_addr) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory"); }
+// (relaxed: what the others have to see by then are barriers, which fence.mbarrier_init has released)
+__device__ __forceinline__ void mx_cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void mx_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float lds_f32(uint32_t addr) { return __uint_as_float(lds32(addr)); }
+// A value to another CTA's shared memory; its barrier there counts the four bytes when they have arrived.
+__device__ __forceinline__ void st_async_f32(uint32_t cluster_addr, float v, uint32_t cluster_bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(cluster_addr), "r"(__float_as_uint(v)), "r"(cluster_bar) : "memory");
+}
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");

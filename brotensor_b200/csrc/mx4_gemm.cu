@@ -234,7 +234,7 @@ static int launch_mx_gemm(const MxParams& p, int64_t x_tiles, size_t smem, cudaS
     int dev = 0;
     B200Q_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        B200Q_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 2048));
+        B200Q_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     const int64_t blocks = x_tiles * p.row_tiles * p.split;
@@ -263,6 +263,9 @@ int launch_mx4_wide(const void* W, const void* W_up, const void* X, const void* 
 static int g_mx4_wide = 1;
 void mx4_set_wide(int v) { g_mx4_wide = v; }
 int mx4_get_wide() { return g_mx4_wide; }
+static int g_mx4_few = 32;
+void mx4_set_few(int v) { g_mx4_few = v; }
+int mx4_get_few() { return g_mx4_few; }
 
 // One matrix (plan == nullptr: M rows of X) or the experts of a plan (buffer laid out for `pairs` pairs and E experts).
 int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K,
@@ -305,17 +308,16 @@ int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* 
     // asked for such that TMEM cannot run out: CTAs that fit an SM by their shared memory fit its 512 columns too.
     const int acc = mats * p.n_cols, sf = 8 * (mats + 1);
     const bool two = acc + 4 * sf <= 256;
-    const int budget = two ? 110 * 1024 : 220 * 1024;
+    const int budget = two ? 110 * 1024 : 222 * 1024;
     p.n_stages = budget / p.stage_bytes;
     if (p.n_stages > kMxMaxStages) p.n_stages = kMxMaxStages;
     const int cols = two ? 256 : 512;
     while (acc + p.n_stages * sf > cols) --p.n_stages;
     p.tmem_cols = (uint32_t)cols;
     size_t smem = (size_t)p.n_stages * p.stage_bytes;
-    const size_t parts = p.split > 1 ? (size_t)mats * p.n_cols * 512 : 0, least = two ? 80 * 1024 : 160 * 1024;
+    const size_t parts = p.split > 1 ? (size_t)mats * p.n_cols * 512 : 0;
     if (smem < parts) smem = parts;
-    if (smem < least) smem = least;
-    smem += 1024;
+    smem = mx_smem_for_tmem(smem + 1024, two ? 256 : 512);
     return mats == 2 ? launch_mx_gemm<2>(p, x_tiles, smem, st) : launch_mx_gemm<1>(p, x_tiles, smem, st);
 }
 

@@ -1,60 +1,10 @@
 // MXFP4 images: made from dense rows (quantise) or from a file's blocks (pack), and read back (dequantise).
-//
-// Quantisation (OCP Microscaling Formats specification 1.0, 6.3): a block's exponent is floor(log2(largest magnitude)) - 2, which puts
-// the largest magnitude into [4, 8); elements are divided by that power of two - exact in FP32 - and rounded to the nearest E2M1
-// value, ties to the even one, magnitudes beyond 6 to 6. A block with an infinity or a NaN becomes NaN as a whole (e = 255), one of zeros e = 0.
 // Bound by memory: 2 or 4 bytes in, 17/32 of a byte out per element, nothing is read twice.
 #include "mx4_common.cuh"
 
 namespace b200q {
 
 constexpr int kQuantThreads = 256;
-
-// Eight neighbouring elements in FP32.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = ld_dep_f4(p), b = ld_dep_f4(p + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        union {
-            uint4 q;
-            T e[8];
-        } u;
-        u.q = ld_dep_u4(p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(u.e[i]);
-    }
-}
-
-// A quad of lanes holds a block, eight elements each: returns the lane's eight nibbles and the block's scale byte.
-__device__ __forceinline__ uint32_t quantise8(const float (&v)[8], uint32_t& scale) {
-    uint32_t top = 0;  // magnitudes as bits compare like magnitudes, infinities and NaNs above all
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int be = (int)(top >> 23);  // 0: a zero or a subnormal, below 2^-126 - the smallest scale serves
-    if (be == 255) {
-        scale = 255u;
-        return 0u;
-    }
-    const int e = max(be - 2, 0);  // biased exponent of the scale
-    scale = (uint32_t)e;
-    // 1 / scale = 2^(127 - e), 127 - e in -125 .. 127
-    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-    uint32_t out;
-    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
-        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
-        : "=r"(out)
-        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
-    return out;
-}
 
 // Blocks of the three kernels cover a patch of rows x column tiles: of a block's eight warps 2^wide stand side by side along a row, the others
 // on the rows below, and each takes `kBatch` neighbouring column tiles, whose loads are in flight together. No index needs a division (with
@@ -85,13 +35,13 @@ __global__ void __launch_bounds__(kQuantThreads) mx4_quantise_kernel(const T* x,
     for (int u = 0; u < kBatch; ++u) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
-        if ((at.kt + u) * kMxTileK + 8 * lane < K) load8(src + u * kMxTileK, v[u]);
+        if ((at.kt + u) * kMxTileK + 8 * lane < K) mx_load8(src + u * kMxTileK, v[u]);
     }
     uint32_t q[kBatch], word[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
         uint32_t sc;
-        q[u] = quantise8(v[u], sc);
+        q[u] = mx_quantise8(v[u], sc);
         // the four scales of the lane's half (blocks 0..3 or 4..7) in one word
         word[u] = sc << (8 * (b & 3));
         word[u] |= __shfl_xor_sync(0xffffffffu, word[u], 4);

@@ -408,6 +408,13 @@ def set_option(key: str, value: int) -> None:
     capi.check(capi.lib().b200q_set_option(key.encode(), value))
 
 
+def get_option(key: str) -> int:
+    import ctypes
+    v = ctypes.c_int(0)
+    capi.check(capi.lib().b200q_get_option(key.encode(), ctypes.byref(v)))
+    return v.value
+
+
 def device_status() -> int:
     """Synchronises; returns 0 or raises if a kernel's bounded wait ran out."""
     import ctypes

@@ -90,12 +90,15 @@ def test_pack_takes_blocks_from_any_byte():
     assert torch.equal(ops.mx4_dequantize(ops.mx4_pack(shifted[5:], 64, 256), 64, 256), ref.matrix(b, 64, 256).float())
 
 
-@pytest.fixture(params=[0, 1, 2], ids=["small tiles", "as routed", "wide tiles"])
+@pytest.fixture(params=["as routed", "small tiles", "wide tiles", "few rows"])
 def route(request):
-    """Both kernels take every call; each is held to the definition whatever the routing rule says."""
-    ops.set_option("mx4_wide", request.param)
+    """Each kernel takes every call (that of few rows, every call of up to 32 of them) and is held to the definition whatever the routing rules say."""
+    was = ops.get_option("mx4_wide"), ops.get_option("mx4_few")
+    ops.set_option("mx4_wide", {"small tiles": 0, "wide tiles": 2}.get(request.param, was[0]))
+    ops.set_option("mx4_few", {"small tiles": 0, "wide tiles": 0, "few rows": 32}.get(request.param, was[1]))
     yield
-    ops.set_option("mx4_wide", 1)
+    ops.set_option("mx4_wide", was[0])
+    ops.set_option("mx4_few", was[1])
 
 
 @pytest.mark.parametrize("M", [1, 2, 16, 17, 100, 128, 129, 300])
