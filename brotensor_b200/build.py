@@ -25,7 +25,7 @@ NVCC_FLAGS = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-
 NVCC_FLAGS = [f for f in NVCC_FLAGS if f != "--use_fast_math=false"]
 
 KERNEL_SOURCES = ["api.cu", "dequant.cu", "repack.cu", "gemv_simple.cu", "gemv_stream.cu", "gemv_dp.cu", "gemv_xr.cu", "gemv_i8.cu", "gemv_hm.cu", "gemv_mb.cu", "gemm_mm.cu", "gemm_tc.cu", "gemm_tc2.cu", "gemm_static.cu",
-                  "mx4_quant.cu", "mx4_gemm.cu", "mx4_wide.cu", "mx4_few.cu", "moe_route.cu", "api_mx4.cu"]
+                  "mx4_quant.cu", "mx4_gemm.cu", "mx4_wide.cu", "moe_route.cu", "api_mx4.cu"]
 
 
 def _newer(src_list, target) -> bool:

@@ -56,7 +56,6 @@ void mx4_set_wide(int v);
 int mx4_get_wide();
 void mx4_set_few(int v);
 int mx4_get_few();
-void few_set(int, int);
 int mm_get_enabled();
 int mb_get_enabled();
 void i8_set_enabled(int v);
@@ -639,7 +638,6 @@ int b200q_set_option(const char* key, int value) {
     else if (!strcmp(key, "gemm_mm")) mm_set_enabled(value);
     else if (!strcmp(key, "mx4_wide")) mx4_set_wide(value);
     else if (!strcmp(key, "mx4_few")) mx4_set_few(value);
-    else if (!strcmp(key, "few_probe")) few_set(value & 15, value >> 4);
     else if (!strcmp(key, "gemv_step_fill")) dp_set_step_fill(value);
     else return fail(B200Q_ERR_BAD_ARG, "set_option: unknown key '%s'", key);
     return B200Q_OK;

@@ -9,10 +9,10 @@ int launch_mx4_quantise(const void* x, int x_dtype, int64_t rows, int K, void* i
 int launch_mx4_dequantise(const void* image, int64_t rows, int K, void* out, int out_dtype, int sms, cudaStream_t st);
 int launch_mx4_pack(const void* blocks, int64_t rows, int64_t count, int K, void* image, cudaStream_t st);
 int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K,
-                    const int* plan, int64_t pairs, int E, int sms, int* status, cudaStream_t st);
-int launch_mx4_few(const void* W, const void* W_up, const void* X, int x_dtype, const void* bias, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
-                   int pairs_per_row, int E, int sms, int* status, cudaStream_t st, bool* taken);
-int mx4_get_few();
+                    const int* plan, int64_t pairs, int E, int early, int sms, int* status, cudaStream_t st);
+int launch_mx4_dense(const void* W, const void* W_up, const void* X, int x_dtype, const void* bias, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
+                   int pairs_per_row, int E, int sms, int* status, cudaStream_t st);
+bool mx4_dense_takes(int64_t rows, int K);
 int launch_moe_topk(const void* logits, int dtype, int64_t tokens, int E, int k, int normalize, float scale, int* ids, float* weights, int sms, cudaStream_t st);
 int launch_moe_plan(const int* ids, int64_t pairs, int E, int* plan, cudaStream_t st);
 int launch_moe_combine(const void* y, int dtype, const int* ids, const float* weights, int64_t tokens, int k, int N, int E, void* out, int sms, cudaStream_t st);
@@ -77,14 +77,12 @@ int b200q_mx4_dequantize(const void* image, int64_t rows, int K, void* out, int 
     return launch_mx4_dequantise(image, rows, K, out, out_dtype, sms, static_cast<cudaStream_t>(stream));
 }
 
-static int gemm_common(const char* op, const void* W, const void* X_image, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, void* stream) {
-    if (!W || !X_image || !Y) return fail(B200Q_ERR_BAD_ARG, "%s: null pointer", op);
-    if (!on(W, 16) || !on(X_image, 16)) return fail(B200Q_ERR_BAD_ARG, "%s: images must be 16-byte aligned", op);
+static int check_product(const char* op, const void* W, const void* X, const void* bias, int bias_dtype, const void* Y, int y_dtype) {
+    if (!W || !X || !Y) return fail(B200Q_ERR_BAD_ARG, "%s: null pointer", op);
+    if (!on(W, 16) || !on(X, 16)) return fail(B200Q_ERR_BAD_ARG, "%s: W and X must be 16-byte aligned", op);
     if (!on(Y, dtype_size(y_dtype))) return fail(B200Q_ERR_BAD_ARG, "%s: Y is not aligned to its element size", op);
     if (bias && !on(bias, dtype_size(bias_dtype))) return fail(B200Q_ERR_BAD_ARG, "%s: the bias is not aligned to its element size", op);
-    int sms, *status;
-    if (int rc = device_facts(&sms, &status)) return rc;
-    return launch_mx4_gemm(W, nullptr, X_image, bias, bias_dtype, Y, y_dtype, M, N, K, nullptr, 0, 0, sms, status, static_cast<cudaStream_t>(stream));
+    return B200Q_OK;
 }
 
 int b200q_mx4_gemm(const void* W, const void* X_image, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, void* stream) {
@@ -92,13 +90,16 @@ int b200q_mx4_gemm(const void* W, const void* X_image, const void* bias, int bia
     if (int rc = check_k("mx4_gemm", K)) return rc;
     if (M < 0 || N < 0) return fail(B200Q_ERR_BAD_ARG, "mx4_gemm: negative shape (M %d, N %d)", M, N);
     if (M == 0 || N == 0) return B200Q_OK;
-    return gemm_common("mx4_gemm", W, X_image, bias, bias_dtype, Y, y_dtype, M, N, K, stream);
+    if (int rc = check_product("mx4_gemm", W, X_image, bias, bias_dtype, Y, y_dtype)) return rc;
+    int sms, *status;
+    if (int rc = device_facts(&sms, &status)) return rc;
+    return launch_mx4_gemm(W, nullptr, X_image, bias, bias_dtype, Y, y_dtype, M, N, K, nullptr, 0, 0, 0, sms, status, static_cast<cudaStream_t>(stream));
 }
 
-size_t b200q_mx4_linear_workspace_bytes(int M, int K) { return b200q_mx4_image_bytes(M, K); }
+size_t b200q_mx4_linear_workspace_bytes(int M, int K) { return mx4_dense_takes(M, K) ? 0 : b200q_mx4_image_bytes(M, K); }
 
 static int check_ws(const char* op, const void* ws, size_t ws_bytes, size_t need) {
-    if (!ws || !on(ws, 256) || ws_bytes < need) return fail(B200Q_ERR_WORKSPACE, "%s: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", op, need, ws ? ws_bytes : (size_t)0);
+    if (need && (!ws || !on(ws, 256) || ws_bytes < need)) return fail(B200Q_ERR_WORKSPACE, "%s: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", op, need, ws ? ws_bytes : (size_t)0);
     return B200Q_OK;
 }
 
@@ -108,22 +109,14 @@ int b200q_mx4_linear(const void* W, const void* X, int x_dtype, const void* bias
     if (int rc = check_k("mx4_linear", K)) return rc;
     if (M < 0 || N < 0) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: negative shape (M %d, N %d)", M, N);
     if (M == 0 || N == 0) return B200Q_OK;
-    if (!X) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: null pointer");
-    if (!on(X, 16)) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: X must be 16-byte aligned");
-    if (!W || !Y) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: null pointer");
+    if (int rc = check_product("mx4_linear", W, X, bias, x_dtype, Y, y_dtype)) return rc;
     if (int rc = check_ws("mx4_linear", ws, ws_bytes, b200q_mx4_linear_workspace_bytes(M, K))) return rc;
-    if (!on(W, 16)) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: images must be 16-byte aligned");
-    if (!on(Y, dtype_size(y_dtype))) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: Y is not aligned to its element size");
-    if (bias && !on(bias, dtype_size(x_dtype))) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: the bias is not aligned to its element size");
-    if (M <= mx4_get_few()) {
-        int sms, *status;
-        if (int rc = device_facts(&sms, &status)) return rc;
-        bool taken;
-        if (int rc = launch_mx4_few(W, nullptr, X, x_dtype, bias, Y, y_dtype, M, N, K, nullptr, 0, 1, 0, sms, status, static_cast<cudaStream_t>(stream), &taken)) return rc;
-        if (taken) return B200Q_OK;
-    }
-    if (int rc = b200q_mx4_quantize(X, x_dtype, M, K, ws, stream)) return rc;
-    return gemm_common("mx4_linear", W, ws, bias, x_dtype, Y, y_dtype, M, N, K, stream);
+    int sms, *status;
+    if (int rc = device_facts(&sms, &status)) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (mx4_dense_takes(M, K)) return launch_mx4_dense(W, nullptr, X, x_dtype, bias, Y, y_dtype, M, N, K, nullptr, 0, 1, 0, sms, status, st);
+    if (int rc = launch_mx4_quantise(X, x_dtype, M, K, ws, nullptr, 1, sms, st)) return rc;
+    return launch_mx4_gemm(W, nullptr, ws, bias, x_dtype, Y, y_dtype, M, N, K, nullptr, 0, 0, 1, sms, status, st);
 }
 
 size_t b200q_moe_plan_bytes(int64_t tokens, int k, int E) {
@@ -158,7 +151,7 @@ int b200q_moe_route(const void* logits, int dtype, int64_t tokens, int E, int k,
 
 size_t b200q_moe_mx4_workspace_bytes(int64_t tokens, int k, int E, int K) {
     if (tokens < 0 || k < 1 || k > kMaxExpertsPerToken || E < 1 || E > kMaxExperts || K <= 0 || K % 32) return 0;
-    return (size_t)moe_plan_layout(tokens * k, E).max_tiles * mx_k_tiles(K) * kMxTileBytes;
+    return mx4_dense_takes(tokens * k, K) ? 0 : (size_t)moe_plan_layout(tokens * k, E).max_tiles * mx_k_tiles(K) * kMxTileBytes;
 }
 
 static int experts_common(const char* op, const void* W, const void* W_up, const void* X, int x_dtype, int x_per_pair, const void* plan, const void* bias, void* Y,
@@ -168,24 +161,19 @@ static int experts_common(const char* op, const void* W, const void* W_up, const
     if (int rc = check_experts(op, tokens, k, E)) return rc;
     if (N < 0) return fail(B200Q_ERR_BAD_ARG, "%s: negative N (%d)", op, N);
     if (tokens == 0 || N == 0) return B200Q_OK;
-    if (!W || !X || !plan || !Y) return fail(B200Q_ERR_BAD_ARG, "%s: null pointer", op);
-    if (!on(W, 16) || !on(W_up, 16) || !on(X, 16) || !on(plan, 16)) return fail(B200Q_ERR_BAD_ARG, "%s: images, X and the plan must be 16-byte aligned", op);
-    if (!on(Y, dtype_size(y_dtype))) return fail(B200Q_ERR_BAD_ARG, "%s: Y is not aligned to its element size", op);
-    if (bias && !on(bias, dtype_size(x_dtype))) return fail(B200Q_ERR_BAD_ARG, "%s: the bias is not aligned to its element size", op);
+    if (!plan) return fail(B200Q_ERR_BAD_ARG, "%s: null pointer", op);
+    if (int rc = check_product(op, W, X, bias, x_dtype, Y, y_dtype)) return rc;
+    if (!on(W_up, 16) || !on(plan, 16)) return fail(B200Q_ERR_BAD_ARG, "%s: images and the plan must be 16-byte aligned", op);
     if (int rc = check_ws(op, ws, ws_bytes, b200q_moe_mx4_workspace_bytes(tokens, k, E, K))) return rc;
     int sms, *status;
     if (int rc = device_facts(&sms, &status)) return rc;
     const int64_t pairs = tokens * k;
     const int* pl = static_cast<const int*>(plan);
-    if (pairs <= mx4_get_few()) {
-        bool taken;
-        if (int rc = launch_mx4_few(W, W_up, X, x_dtype, bias, Y, y_dtype, 0, N, K, pl, pairs, x_per_pair ? 1 : k, E, sms, status, static_cast<cudaStream_t>(stream), &taken)) return rc;
-        if (taken) return B200Q_OK;
-    }
-    const int* place = pl + moe_plan_layout(pairs, E).place;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (mx4_dense_takes(pairs, K)) return launch_mx4_dense(W, W_up, X, x_dtype, bias, Y, y_dtype, 0, N, K, pl, pairs, x_per_pair ? 1 : k, E, sms, status, st);
+    const int* place = pl + moe_plan_layout(pairs, E).place;
     if (int rc = launch_mx4_quantise(X, x_dtype, x_per_pair ? pairs : tokens, K, ws, place, x_per_pair ? 1 : k, sms, st)) return rc;
-    return launch_mx4_gemm(W, W_up, ws, bias, x_dtype, Y, y_dtype, 0, N, K, pl, pairs, E, sms, status, st);
+    return launch_mx4_gemm(W, W_up, ws, bias, x_dtype, Y, y_dtype, 0, N, K, pl, pairs, E, 1, sms, status, st);
 }
 
 int b200q_moe_mx4_linear(const void* W, const void* X, int x_dtype, int x_per_pair, const void* plan, const void* bias, void* Y, int y_dtype, int64_t tokens, int k,

@@ -118,6 +118,18 @@ __device__ __forceinline__ uint32_t mx_quantise8(const float (&v)[8], uint32_t& 
     return out;
 }
 
+// Loads that do not go through the L1, for what is read ahead of griddepcontrol.wait.
+__device__ __forceinline__ uint4 ld_l2_u4(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_l2_u32(const void* p) {
+    uint32_t v;
+    asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+
 // ---- tcgen05 kind::mxf4 -----------------------------------------------------------------------------------------
 // Operand without swizzle, rows of 16 bytes in groups of eight (128 bytes): the layout of a piece of scales.
 __device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
@@ -176,11 +188,6 @@ __device__ __forceinline__ float lds_f32(uint32_t addr) { return __uint_as_float
 __device__ __forceinline__ void st_async_f32(uint32_t cluster_addr, float v, uint32_t cluster_bar) {
     asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(cluster_addr), "r"(__float_as_uint(v)), "r"(cluster_bar) : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
 
 // The roles that issue copies and MMAs run as whole warps with one elected lane at the instructions themselves: control flow, addresses and
 // descriptors are then uniform for the compiler. (As code of one lane, every operand went through a conversion to a uniform register
@@ -192,9 +199,9 @@ __device__ __forceinline__ bool mx_elect() {
     return p != 0;
 }
 // Bounded wait of a whole warp; false on all lanes once the CTA has given up.
-__device__ __forceinline__ bool mx_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+__device__ __forceinline__ bool mx_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code, uint64_t limit_ns = kWaitLimitNs) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, wait_or_abort_slow(bar, parity, abort_flag, status, code, kWaitLimitNs) && !*abort_flag);
+    return __all_sync(0xffffffffu, wait_or_abort_slow(bar, parity, abort_flag, status, code, limit_ns) && !*abort_flag);
 }
 
 // silu(g) * u. exp2f of a rounded product: |g| 2^-24 off relative, which only negative g feel, where silu is small; the quotient within two units.

@@ -1,59 +1,79 @@
 // Products of MXFP4 images on the block-scaled tensor cores (tcgen05 kind::mxf4):
 //   Y(M,N) = X(M,K) W(N,K)^T (+ bias),  both operands E2M1 with one E8M0 scale per 32 columns, FP32 accumulation in TMEM,
 // for one matrix (a projection) or, over the tiles of a MoePlan, for the matrices of many experts; with two matrices the
-// result is silu(gate) * up.
+// result is silu(gate) * up. This kernel is for few activation rows (mx4_wide.cu: many).
 //
 // A CTA owns 128 weight rows (the MMA's M, TMEM lanes) and up to 128 activation rows (its N, TMEM columns), so that a
-// product of a few rows wastes little and results of one activation row leave as contiguous stores. Per 256 columns a
-// stage holds one tile of each image - one bulk copy each, scales included - and costs two tcgen05.cp per operand (128
-// columns' scales to TMEM) and four MMAs of 64 columns. Products and sums are exact or FP32: the operands need no decoding.
-//   warp 0      one thread streams the stages through the ring
-//   warp 1      TMEM allocation; one thread issues copies of scales, MMAs and commits
-//   warps 2..5  epilogue (each its lane quarter)
-// Few tiles: the k range is cut over the CTAs of a cluster of up to eight, whose partial sums meet through distributed
-// shared memory in rank order - no workspace, no atomics, the same result on every run.
-// All waits are bounded as in the other kernels; on a timeout the CTA records a status code, still takes part in the
-// cluster barriers, frees its TMEM and returns.
+// product of a few rows wastes little. Per 256 columns a stage holds one tile of each image - one bulk copy each, scales included -
+// and costs two tcgen05.cp per operand (128 columns' scales to TMEM) and four MMAs of 64 columns. Nothing is decoded.
+// Bound by the weights' way from HBM (17 bits of 32 per weight); everything else has to hide behind it.
+//   warp 0       loader    warp 1  TMEM, scales, MMAs    warps 2..5  epilogue (each its lane quarter)
+//
+// XT = void: X is an image (mx4_quant.cu has made it just before). Otherwise X is dense, of at most 16 rows (decode), and warps 2..9 quantise the CTA's
+// part of it first - the same values, kept in shared memory only: a projection is one launch, without a workspace.
+//
+// Few tiles: the k range is cut over the CTAs of a cluster of up to eight. Each rank sends its sums of a slice of the weight rows to the rank
+// that adds the slice up, in rank order - no workspace, no atomics, the same result on every run. (With the sums fetched from the
+// others' shared memory between two cluster barriers a launch took 1.5 us more.)
+//
+// All waits are bounded as in the other kernels; on a timeout the CTA records a status code, sends zeros, frees its TMEM and returns.
+#include <type_traits>
+
 #include "mx4_common.cuh"
 
 namespace b200q {
 
-constexpr int kMxThreads = 192, kMxEpilogueWarp0 = 2;
-constexpr int kMxMaxStages = 12;
+constexpr int kMxMaxStages = 12, kMxDenseRows = 16;
+constexpr int kMxDenseTiles = 32;  // dense X: most column tiles of a CTA (activations 96 KB, beside three gated stages 105 KB)
+constexpr int kMxQuantWarps = 8;  // dense X: warps that quantise (four of them then have the epilogue)
+template <typename XT>
+constexpr bool kIsImage = std::is_same_v<XT, void>;
+template <typename XT>
+constexpr int kMxThreads = 64 + 32 * (kIsImage<XT> ? 4 : kMxQuantWarps);
 
 struct MxParams {
-    const uint8_t* W;      // image of the (gate) weights; expert e's lies e * w_expert_bytes behind
-    const uint8_t* W_up;   // image of the up weights, or nullptr
-    const uint8_t* X;      // image of the activations
+    const uint8_t* W;
+    const uint8_t* W_up;
+    const void* X;         // image or dense rows
     const void* bias;      // N values (per expert), or nullptr
     void* Y;
     int* status;
     size_t w_expert_bytes;
-    const int4* tiles;     // grouped: {expert, first place, rows, 0} of each tile of X; nullptr: one matrix, M rows
+    const int4* tiles;   // grouped: {expert, first place, rows, 0}; nullptr: one matrix, M rows
     const int* n_tiles;
-    const int* order;      // grouped: place -> row of Y
+    const int* order;    // grouped: place -> pair, the row of Y
+    int pairs_per_row;   // grouped, dense X: pairs that share a row of X (1: X has a row for each pair)
     int M, N, K;
-    int row_tiles, k_tiles, split, split_tiles;  // CTA rank r of a cluster of `split` works on k tiles [r * split_tiles, ..)
+    int k_tiles, split_log2, split_tiles;  // CTA rank r of a cluster of 2^split_log2 works on column tiles [r * split_tiles, ..)
     int bias_dtype, y_dtype;
-    int n_cols;            // accumulator columns per matrix (activation rows of a full tile, a multiple of 16)
+    int n_cols;          // accumulator columns of a matrix: activation rows of a full tile, a multiple of 16
     int n_stages, stage_bytes;
+    int experts;
+    int early;           // the predecessor writes neither weights nor plan (it is the quantisation): they are read ahead of its end
     uint32_t tmem_cols;
 };
 
-template <int MATS>  // weight matrices: 1, or 2 for silu(gate) * up
-__global__ void __launch_bounds__(kMxThreads) mx4_gemm_kernel(const MxParams p) {
+template <int MATS, typename XT>
+__global__ void __launch_bounds__(kMxThreads<XT>, kIsImage<XT> ? 2 : 3) mx4_gemm_kernel(const MxParams p) {
+    constexpr uint32_t kWBytes = MATS * kMxTileBytes;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    __shared__ uint64_t bar_full[kMxMaxStages], bar_empty[kMxMaxStages], bar_accum;
+    __shared__ uint64_t bar_full[kMxMaxStages], bar_empty[kMxMaxStages], bar_x, bar_accum, bar_parts;
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
-    __shared__ int out_row[kMxTileRows];  // row of Y of each activation row of the tile
+    __shared__ int row_of[kMxTileRows];  // row of Y of each activation row of the tile
 
+    // Most of this kernel's time beside the weights' is latency, so what can be worked out ahead of a wait is, and nothing divides.
     const int tid = threadIdx.x, warp = mx_uniform_warp(), lane = tid & 31;
-    const uint32_t crank = p.split > 1 ? mx_cluster_rank() : 0u;
-    const int64_t work = (int64_t)(blockIdx.x / (unsigned)p.split);
-    const int64_t x_tile = work / p.row_tiles;
-    const int row_tile = (int)(work - x_tile * p.row_tiles);
+    const int split = 1 << p.split_log2, mine_log2 = 7 - p.split_log2, mine = 1 << mine_log2;
+    const uint32_t crank = p.split_log2 ? mx_cluster_rank() : 0u;
+    const int x_tile = (int)blockIdx.y, row_tile = (int)blockIdx.x >> p.split_log2;
+    const int kt0 = (int)crank * p.split_tiles, share = max(min(p.split_tiles, p.k_tiles - kt0), 0);
+    // The activations of a column tile: 1024 bytes of scales, n_cols rows of 128 bytes. An image's are part of the stage; dense ones lie
+    // behind the ring for all of the CTA's column tiles. Last the parts: see the epilogue.
+    const uint32_t x_step = (uint32_t)p.n_cols * 128u + kMxSfBytes, x_base = sbase + (uint32_t)(p.n_stages * p.stage_bytes);
+    const uint32_t parts = x_base + (kIsImage<XT> ? 0u : (uint32_t)p.split_tiles * x_step);
+    const size_t w_at = mx_tile_offset(row_tile, kt0, p.k_tiles);
 
     if (tid == 0) {
         abort_flag = 0;
@@ -61,7 +81,9 @@ __global__ void __launch_bounds__(kMxThreads) mx4_gemm_kernel(const MxParams p) 
             mbar_init(smem_u32(&bar_full[s]), 1);
             mbar_init(smem_u32(&bar_empty[s]), 1);
         }
+        if (!kIsImage<XT>) mbar_init(smem_u32(&bar_x), kMxQuantWarps);
         mbar_init(smem_u32(&bar_accum), 1);
+        mbar_init(smem_u32(&bar_parts), 1);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -69,54 +91,74 @@ __global__ void __launch_bounds__(kMxThreads) mx4_gemm_kernel(const MxParams p) 
         tmem_relinquish();
     }
     grid_dep_launch();
+    // The L2 hears about the weights while the predecessor still runs. Whose they are in a grouped product the plan says, which the predecessor
+    // may be writing: a hint may be wrong, so it is only checked to lie inside the weights.
+    if (warp == 0 && share > 0 && !p.early) {
+        int e = 0;
+        if (p.tiles) e = (unsigned)x_tile < ld_l2_u32(p.n_tiles) ? (int)ld_l2_u32(&p.tiles[x_tile].x) : -1;
+        if ((unsigned)e < (unsigned)p.experts && mx_elect()) {
+            const size_t at = (size_t)e * p.w_expert_bytes + w_at;
+            bulk_prefetch_l2(p.W + at, (uint32_t)share * kMxTileBytes);
+            if (MATS == 2) bulk_prefetch_l2(p.W_up + at, (uint32_t)share * kMxTileBytes);
+        }
+        __syncwarp();
+    }
     tc_fence_before();
     __syncthreads();
+    if (p.split_log2) mx_cluster_arrive();  // waited for before the first sums are sent: by then every CTA's barriers exist
     tc_fence_after();
-    grid_dep_wait();
     const uint32_t tmem_base = tmem_base_slot;
+    if (!p.early || warp != 0) grid_dep_wait();
 
-    // what this CTA works on; the same for all CTAs of a cluster
-    int rows, expert = 0, first = 0;
+    int rows = min(p.M - x_tile * kMxTileRows, kMxTileRows), expert = 0, first = x_tile * kMxTileRows;
     if (p.tiles) {
-        rows = 0;
-        if (x_tile < (int64_t)(int)ld_dep_u32(p.n_tiles)) {
-            const uint4 t = ld_dep_u4(p.tiles + x_tile);
-            expert = (int)t.x;
-            first = (int)t.y;
-            rows = (int)t.z;
-        }
-        for (int i = tid; i < rows; i += kMxThreads) out_row[i] = (int)ld_dep_u32(p.order + first + i);
-    } else {
-        rows = (int)min((int64_t)kMxTileRows, (int64_t)p.M - x_tile * kMxTileRows);
-        for (int i = tid; i < rows; i += kMxThreads) out_row[i] = (int)(x_tile * kMxTileRows) + i;
+        const int n_tiles = (int)ld_l2_u32(p.n_tiles);
+        const uint4 t = ld_l2_u4(p.tiles + x_tile);  // (there is room for every x_tile of the grid)
+        const bool is_tile = x_tile < n_tiles;
+        expert = is_tile ? (int)t.x : 0;
+        first = (int)t.y;
+        rows = is_tile ? (int)t.z : 0;
     }
-    __syncthreads();
-    const int kt0 = (int)crank * p.split_tiles, n_kt = rows > 0 ? min(p.split_tiles, p.k_tiles - kt0) : 0;
-    const int n_mma = (rows + 15) & ~15;
-    int issued = 0;  // warp 0's thread: stages requested
+    const int n_kt = rows > 0 ? share : 0, n_mma = kIsImage<XT> ? (rows + 15) & ~15 : kMxDenseRows;
+    int issued = 0;
+    bool live = true;
 
-    const uint32_t sf_col0 = (uint32_t)(MATS * p.n_cols);  // scales behind the accumulators: per stage 8 columns for each matrix, 8 for X
     if (warp == 0) {
-        const uint8_t* w0 = p.W + (size_t)expert * p.w_expert_bytes + mx_tile_offset(row_tile, kt0, p.k_tiles);
-        const uint8_t* w1 = MATS == 2 ? p.W_up + (size_t)expert * p.w_expert_bytes + mx_tile_offset(row_tile, kt0, p.k_tiles) : nullptr;
-        const uint8_t* x = p.X + mx_tile_offset(x_tile, kt0, p.k_tiles);
+        const size_t at = (size_t)expert * p.w_expert_bytes + w_at;
+        const uint8_t *w0 = p.W + at, *w1 = MATS == 2 ? p.W_up + at : nullptr;
         const uint32_t x_bytes = (uint32_t)n_mma * 128u;
+        const uint8_t* x = kIsImage<XT> ? static_cast<const uint8_t*>(p.X) + mx_tile_offset(x_tile, kt0, p.k_tiles) : nullptr;
+        auto load_w = [&](int kt, uint32_t dst, uint32_t full) {
+            mbar_arrive_expect_tx(full, kWBytes + (kIsImage<XT> ? x_bytes + kMxSfBytes : 0u));
+            bulk_g2s(dst, w0 + (size_t)kt * kMxTileBytes, kMxTileBytes, full);
+            if (MATS == 2) bulk_g2s(dst + kMxTileBytes, w1 + (size_t)kt * kMxTileBytes, kMxTileBytes, full);
+        };
+        auto load_x = [&](int kt, uint32_t dst, uint32_t full) {
+            if constexpr (kIsImage<XT>) {
+                const uint8_t* src = x + (size_t)kt * kMxTileBytes;
+                bulk_g2s(dst + kWBytes + kMxSfBytes, src, x_bytes, full);
+                bulk_g2s(dst + kWBytes, src + kMxQBytes, kMxSfBytes, full);
+            }
+        };
+        // The first stages' weights, then - behind the predecessor, whose results they are - the activations
+        const int head = min(n_kt, p.n_stages);
+        if (mx_elect())
+            for (int kt = 0; kt < head; ++kt) load_w(kt, sbase + kt * p.stage_bytes, smem_u32(&bar_full[kt]));
+        __syncwarp();
+        if (p.early) grid_dep_wait();
+        if (kIsImage<XT> && mx_elect())
+            for (int kt = 0; kt < head; ++kt) load_x(kt, sbase + kt * p.stage_bytes, smem_u32(&bar_full[kt]));
+        __syncwarp();
+        issued = head;
         int slot = 0;
-        uint32_t phase = 1;
-        for (int kt = 0; kt < n_kt; ++kt) {
+        uint32_t phase = 0;
+        for (int kt = head; kt < n_kt; ++kt) {
             if (!mx_warp_wait(smem_u32(&bar_empty[slot]), phase, &abort_flag, p.status, kDevTimeoutEmpty)) break;
-            const uint32_t full = smem_u32(&bar_full[slot]), dst = sbase + slot * p.stage_bytes;
             if (mx_elect()) {
-                mbar_arrive_expect_tx(full, MATS * kMxTileBytes + x_bytes + kMxSfBytes);
-                bulk_g2s(dst, w0, kMxTileBytes, full);
-                if (MATS == 2) bulk_g2s(dst + kMxTileBytes, w1, kMxTileBytes, full);
-                bulk_g2s(dst + MATS * kMxTileBytes + kMxSfBytes, x, x_bytes, full);
-                bulk_g2s(dst + MATS * kMxTileBytes, x + kMxQBytes, kMxSfBytes, full);
+                load_w(kt, sbase + slot * p.stage_bytes, smem_u32(&bar_full[slot]));
+                load_x(kt, sbase + slot * p.stage_bytes, smem_u32(&bar_full[slot]));
             }
             __syncwarp();
-            w0 += kMxTileBytes;
-            if (MATS == 2) w1 += kMxTileBytes;
-            x += kMxTileBytes;
             ++issued;
             if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
         }
@@ -124,112 +166,200 @@ __global__ void __launch_bounds__(kMxThreads) mx4_gemm_kernel(const MxParams p) 
         int slot = 0;
         uint32_t phase = 0;
         const uint32_t id0 = instr_desc_mxf4(kMxTileRows, n_mma, 0), id2 = instr_desc_mxf4(kMxTileRows, n_mma, 2);
-        for (int kt = 0; kt < n_kt; ++kt) {
-            if (!mx_warp_wait(smem_u32(&bar_full[slot]), phase, &abort_flag, p.status, kDevTimeoutFull)) break;
-            tc_fence_after();
-            const uint32_t st = sbase + slot * p.stage_bytes, xs = st + MATS * kMxTileBytes;
-            const uint32_t sf = tmem_base + sf_col0 + (uint32_t)(slot * 8 * (MATS + 1));
-            const int left = p.K - (kt0 + kt) * kMxTileK;  // columns beyond K are zeros: whole steps of them are left out
-            if (mx_elect()) {
+        if (n_kt > 0 && (kIsImage<XT> || mx_warp_wait(smem_u32(&bar_x), 0, &abort_flag, p.status, kDevTimeoutFull))) {
+            for (int kt = 0; kt < n_kt; ++kt) {
+                if (!mx_warp_wait(smem_u32(&bar_full[slot]), phase, &abort_flag, p.status, kDevTimeoutFull)) break;
+                tc_fence_after();
+                const uint32_t st = sbase + slot * p.stage_bytes, xs = kIsImage<XT> ? st + kWBytes : x_base + (uint32_t)kt * x_step;
+                const uint32_t sf = tmem_base + (uint32_t)(MATS * p.n_cols + slot * 8 * (MATS + 1));
+                const int left = p.K - (kt0 + kt) * kMxTileK;
+                if (mx_elect()) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int m = 0; m < MATS; ++m) tmem_cp_scales<1>(sf + 8 * m + 4 * h, smem_desc_scales(st + m * kMxTileBytes + kMxQBytes + 512 * h));
-                    tmem_cp_scales<1>(sf + 8 * MATS + 4 * h, smem_desc_scales(xs + 512 * h));
+                        for (int m = 0; m < MATS; ++m) tmem_cp_scales<1>(sf + 8 * m + 4 * h, smem_desc_scales(st + m * kMxTileBytes + kMxQBytes + 512 * h));
+                        tmem_cp_scales<1>(sf + 8 * MATS + 4 * h, smem_desc_scales(xs + 512 * h));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (64 * j < left) {
+#pragma unroll
+                            for (int m = 0; m < MATS; ++m)
+                                umma_mxf4<1>(tmem_base + m * p.n_cols, smem_desc_sw128(st + m * kMxTileBytes + 32 * j), smem_desc_sw128(xs + kMxSfBytes + 32 * j), j & 1 ? id2 : id0,
+                                             sf + 8 * m + 4 * (j >> 1), sf + 8 * MATS + 4 * (j >> 1), (kt | j) != 0);
+                        }
+                    umma_commit(smem_u32(&bar_empty[slot]));
+                    if (kt + 1 == n_kt) umma_commit(smem_u32(&bar_accum));
                 }
+                __syncwarp();
+                if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
+            }
+        }
+    } else {
+        const int w = warp - 2;
+        if (w < 4) {
+            const int i = w * 32 + lane;
+            if (i < rows) row_of[i] = p.tiles ? (int)ld_l2_u32(p.order + first + i) : first + i;
+        }
+        if constexpr (!kIsImage<XT>) {
+        if (n_kt > 0) {
+            // lane r: the row of X of activation row r
+            int my_src = lane;
+            if (p.tiles && lane < rows) {
+                my_src = (int)ld_l2_u32(p.order + first + lane);
+                if (p.pairs_per_row > 1) my_src /= p.pairs_per_row;
+            }
+            // A warp quantises 256 columns of a row at a time, lane 4 b + s elements 8 s .. 8 s + 7 of block b, with the next row's loads under way.
+            // Up to eight column tiles the warps stand on one each, several rows abreast.
+            const int b = lane >> 2, s = lane & 3;
+            const int abreast = n_kt < kMxQuantWarps ? kMxQuantWarps / n_kt : 1, r0 = w / n_kt;
+            if (r0 < abreast) {
+                for (int kt = w - r0 * n_kt; kt < n_kt; kt += kMxQuantWarps) {
+                    const int k = (kt0 + kt) * kMxTileK + 8 * lane;
+                    const XT* x = static_cast<const XT*>(p.X) + k;
+                    const uint32_t at = x_base + (uint32_t)kt * x_step, to = at + kMxSfBytes + 4 * s, sc_to = at + (uint32_t)((lane >> 4) * 512);
+                    float v[8], next[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (64 * j < left) {
-                        const uint64_t xd = smem_desc_sw128(xs + kMxSfBytes + 32 * j);
+                    for (int j = 0; j < 8; ++j) v[j] = next[j] = 0.f;
+                    int64_t src = __shfl_sync(0xffffffffu, my_src, r0 & 31);
+                    if (r0 < rows && k < p.K) mx_load8(x + src * p.K, v);
+                    for (int r = r0; r < rows; r += abreast) {
+                        src = __shfl_sync(0xffffffffu, my_src, (r + abreast) & 31);
+                        if (r + abreast < rows && k < p.K) mx_load8(x + src * p.K, next);
+                        uint32_t sc;
+                        const uint32_t q = mx_quantise8(v, sc);
+                        uint32_t word = sc << (8 * (b & 3));
+                        word |= __shfl_xor_sync(0xffffffffu, word, 4);
+                        word |= __shfl_xor_sync(0xffffffffu, word, 8);
+                        sts32(to + (uint32_t)(r >> 3) * 1024u + (uint32_t)(r & 7) * 128u + ((uint32_t)(b ^ (r & 7)) << 4), q);
+                        if ((lane & 15) == 0) sts32(sc_to + (uint32_t)r * 16u, word);
 #pragma unroll
-                        for (int m = 0; m < MATS; ++m)
-                            umma_mxf4<1>(tmem_base + m * p.n_cols, smem_desc_sw128(st + m * kMxTileBytes + 32 * j), xd, j & 1 ? id2 : id0,
-                                         sf + 8 * m + 4 * (j >> 1), sf + 8 * MATS + 4 * (j >> 1), (kt | j) != 0);
+                        for (int j = 0; j < 8; ++j) v[j] = next[j];
                     }
                 }
-                umma_commit(smem_u32(&bar_empty[slot]));
             }
+            fence_proxy_async_smem();  // generic-proxy writes -> visible to the tensor cores
             __syncwarp();
-            if (++slot == p.n_stages) { slot = 0; phase ^= 1; }
+            if (lane == 0) mbar_arrive(smem_u32(&bar_x));
         }
-        if (rows > 0 && mx_elect()) umma_commit(smem_u32(&bar_accum));
-        __syncwarp();
+        }
+        if (w < 4) asm volatile("bar.sync 1, 128;" ::: "memory");  // row_of is complete
     }
-    // ---- epilogue
-    bool live = true;
-    if (warp >= kMxEpilogueWarp0) {
-        if (rows > 0) live = mx_warp_wait(smem_u32(&bar_accum), 0, &abort_flag, p.status, kDevTimeoutMma);
-        tc_fence_after();
+    if (warp >= 2 && warp < 6 && rows > 0) {  // epilogue, each warp its lane quarter
         const int r = (warp & 3) * 32 + lane;  // weight row of the tile = TMEM lane
         const uint32_t tlane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-        const int64_t n = (int64_t)row_tile * kMxTileRows + r;
-        if (live && rows > 0 && p.split == 1) {
+        if (p.split_log2 == 0) {
+            const int64_t n = (int64_t)row_tile * kMxTileRows + r;
             const float bv = p.bias && n < p.N ? load_bias(p.bias, p.bias_dtype, (size_t)expert * p.N + n) : 0.f;
-            for (int c = 0; c < n_mma; c += 16) {
-                uint32_t a[16], b[16];
-                tmem_ld16(tlane + (uint32_t)c, a);
-                if (MATS == 2) tmem_ld16(tlane + (uint32_t)(p.n_cols + c), b);
-                tmem_ld_wait();
-                if (n < p.N) {
+            live = mx_warp_wait(smem_u32(&bar_accum), 0, &abort_flag, p.status, kDevTimeoutMma);
+            tc_fence_after();
+            for (int c = 0; c < rows; c += 16) {
+                uint32_t a[MATS][16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        if (c + j < rows) {
-                            float v = __uint_as_float(a[j]) + bv;
-                            if (MATS == 2) v = silu_times(__uint_as_float(a[j]), __uint_as_float(b[j]));
-                            store_y(p.Y, p.y_dtype, (size_t)out_row[c + j] * p.N + n, v);
-                        }
+                for (int m = 0; m < MATS; ++m) tmem_ld16(tlane + (uint32_t)(m * p.n_cols + c), a[m]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (c + j < rows) {
+                        const size_t row = (size_t)row_of[c + j];
+                        float v = __uint_as_float(a[0][j]) + bv;
+                        if (MATS == 2) v = silu_times(__uint_as_float(a[0][j]), __uint_as_float(a[MATS - 1][j]));
+                        if (live && n < p.N) store_y(p.Y, p.y_dtype, row * p.N + n, v);
                     }
                 }
             }
-        } else if (rows > 0 && p.split > 1) {
-            // partial sums [matrix][activation row][128] over the ring, whose stages are all consumed
-            float* part = reinterpret_cast<float*>(smem_raw + (sbase - smem_u32(smem_raw)));
-            for (int m = 0; m < MATS; ++m)
-                for (int c = 0; c < n_mma; c += 16) {
-                    uint32_t a[16];
-                    tmem_ld16(tlane + (uint32_t)(m * p.n_cols + c), a);
-                    tmem_ld_wait();
+        } else {
+            // Rank q adds up weight rows [q * mine, + mine) of the tile. Every rank sends it its sums of these - parts[rank][matrix][activation
+            // row][mine], weight row r being row r % mine of rank r / mine - and its barrier counts the bytes.
+            if (tid == 64) mbar_arrive_expect_tx(smem_u32(&bar_parts), (uint32_t)(MATS * rows) << 9);
+            const uint32_t to_rank = (uint32_t)(r >> mine_log2);
+            const uint32_t to = mx_map_to_rank(parts + (uint32_t)((((((int)crank * MATS * rows) << mine_log2)) + (r & (mine - 1))) * 4), to_rank);
+            const uint32_t to_bar = mx_map_to_rank(smem_u32(&bar_parts), to_rank);
+            const int t0 = (tid - 64) >> mine_log2;  // this thread's results: activation rows t0, t0 + split, .. of weight row x
+            const int x = (tid - 64) & (mine - 1);
+            const int64_t n = (int64_t)row_tile * kMxTileRows + (int)crank * mine + x;
+            const float bv = p.bias && n < p.N ? load_bias(p.bias, p.bias_dtype, (size_t)expert * p.N + n) : 0.f;
+            mx_cluster_wait();
+            if (n_kt > 0) live = mx_warp_wait(smem_u32(&bar_accum), 0, &abort_flag, p.status, kDevTimeoutMma);
+            tc_fence_after();
+            for (int c = 0; c < rows; c += 16) {
+                uint32_t a[MATS][16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (c + j < rows) part[(m * p.n_cols + c + j) * 128 + r] = live && n_kt > 0 ? __uint_as_float(a[j]) : 0.f;
-                }
-        }
-    }
-    if (p.split > 1) {
-        mx_cluster_sync();
-        // rank q adds up weight rows [q * 128 / split, ..) of the tile, ranks in order
-        const int mine = kMxTileRows / p.split;
-        if (live && rows > 0) {
-            for (int i = tid; i < rows * mine; i += kMxThreads) {
-                const int t = i / mine, r = (int)crank * mine + (i - t * mine);
-                const int64_t n = (int64_t)row_tile * kMxTileRows + r;
-                if (n >= p.N) continue;
-                float s[MATS];
+                for (int m = 0; m < MATS; ++m) tmem_ld16(tlane + (uint32_t)(m * p.n_cols + c), a[m]);
+                tmem_ld_wait();
+                // (a rank that has given up sends zeros: its peers come to an end, the status says that the result is void)
 #pragma unroll
-                for (int m = 0; m < MATS; ++m) {
-                    s[m] = 0.f;
-                    const uint32_t at = sbase + (uint32_t)(((m * p.n_cols + t) * 128 + r) * 4);
-                    for (int q = 0; q < p.split; ++q) s[m] += ld_cluster_f32(mx_map_to_rank(at, (uint32_t)q));
+                for (int j = 0; j < 16; ++j)
+                    if (c + j < rows) {
+#pragma unroll
+                        for (int m = 0; m < MATS; ++m)
+                            st_async_f32(to + ((uint32_t)(m * rows + c + j) << (mine_log2 + 2)), live && n_kt > 0 ? __uint_as_float(a[m][j]) : 0.f, to_bar);
+                    }
+            }
+            // (a peer that waits in vain for something gives up before this does)
+            const bool ok = mx_warp_wait(smem_u32(&bar_parts), 0, &abort_flag, p.status, kDevTimeoutPeer, 4 * kWaitLimitNs);
+            if (ok && n < p.N) {
+                for (int t = t0; t < rows; t += split) {
+                    float s[MATS];
+#pragma unroll
+                    for (int m = 0; m < MATS; ++m) {
+                        s[m] = 0.f;
+                        for (int q = 0; q < split; ++q) s[m] += lds_f32(parts + (uint32_t)((((q * MATS + m) * rows + t) << mine_log2) + x) * 4u);
+                    }
+                    float v = s[0] + bv;
+                    if (MATS == 2) v = silu_times(s[0], s[MATS - 1]);
+                    store_y(p.Y, p.y_dtype, (size_t)row_of[t] * p.N + n, v);
                 }
-                float v = s[0] + (p.bias ? load_bias(p.bias, p.bias_dtype, (size_t)expert * p.N + n) : 0.f);
-                if (MATS == 2) v = silu_times(s[0], s[MATS - 1]);
-                store_y(p.Y, p.y_dtype, (size_t)out_row[t] * p.N + n, v);
             }
         }
-        mx_cluster_sync();  // nobody leaves while its partial sums are read
+    } else if (p.split_log2) {
+        mx_cluster_wait();
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && abort_flag) {  // given up: let the copies in flight land before the CTA's shared memory is given away
         for (int kt = max(issued - p.n_stages, 0); kt < issued; ++kt)
             mbar_wait_bounded(smem_u32(&bar_full[kt % p.n_stages]), (uint32_t)(kt / p.n_stages) & 1u, p.status, kDevTimeoutFull, 1u << 12);
     }
-    if (warp == 1) tmem_dealloc(tmem_base, p.tmem_cols);
+    if (warp == 1) {
+        __syncwarp();
+        tmem_dealloc(tmem_base, p.tmem_cols);
+    }
 }
 
-template <int MATS>
-static int launch_mx_gemm(const MxParams& p, int64_t x_tiles, size_t smem, cudaStream_t st) {
-    auto kern = mx4_gemm_kernel<MATS>;
+template <int MATS, typename XT>
+static int launch_mx_gemm(const MxParams& q, int64_t x_tiles, int64_t rows_most, int sms, cudaStream_t st) {
+    auto kern = mx4_gemm_kernel<MATS, XT>;
+    MxParams p = q;
+    p.n_cols = rows_most >= kMxTileRows ? kMxTileRows : (int)((rows_most + 15) & ~15);
+    const int x_step = p.n_cols * 128 + kMxSfBytes;
+    p.stage_bytes = MATS * kMxTileBytes + (kIsImage<XT> ? x_step : 0);
+    // CTAs to fill the SMs: two of an image's, and of gated dense ones (111 KB each), three of the others (74 KB). K is split while they are fewer and
+    // every share keeps two column tiles or more.
+    const int per_sm = kIsImage<XT> || MATS == 2 ? 2 : 3;
+    const int64_t row_tiles = mx_row_tiles(p.N), tiles = x_tiles * row_tiles;
+    p.split_log2 = 0;
+    while (p.split_log2 < 3 && tiles << (p.split_log2 + 1) <= (int64_t)per_sm * sms && p.k_tiles >= 4 << p.split_log2) ++p.split_log2;
+    if (!kIsImage<XT>)  // every share's activations have to fit beside three stages
+        while ((p.k_tiles + (1 << p.split_log2) - 1) >> p.split_log2 > kMxDenseTiles) ++p.split_log2;
+    const int split = 1 << p.split_log2;
+    p.split_tiles = (p.k_tiles + split - 1) / split;
+    const int fixed = (kIsImage<XT> ? 0 : p.split_tiles * x_step) + (split > 1 ? MATS * p.n_cols * 512 : 0);  // activations, parts
+    if (tiles * split > 2147483647LL || x_tiles > 65535) return fail(B200Q_ERR_UNSUPPORTED, "mx4: %lld x %lld tiles are more than one launch takes", (long long)x_tiles, (long long)row_tiles);
+    // Shared memory of an SM's `per_sm` CTAs; of fewer where three stages would not fit. The stages' scales take TMEM columns behind the accumulators.
+    const int acc = MATS * p.n_cols, sf = 8 * (MATS + 1);
+    int budget = per_sm == 3 ? 74 * 1024 : 111 * 1024;
+    if (fixed + 3 * p.stage_bytes > budget) budget = 111 * 1024;
+    if (fixed + 3 * p.stage_bytes > budget || acc + 3 * sf > 256) budget = 222 * 1024;
+    p.n_stages = (budget - fixed) / p.stage_bytes;
+    if (p.n_stages > kMxMaxStages) p.n_stages = kMxMaxStages;
+    if (p.n_stages > p.split_tiles) p.n_stages = p.split_tiles;
+    const int most = budget == 222 * 1024 ? 512 : 256;
+    while (acc + p.n_stages * sf > most) --p.n_stages;
+    p.tmem_cols = 32u;
+    while ((int)p.tmem_cols < acc + p.n_stages * sf) p.tmem_cols *= 2;
+    const size_t smem = mx_smem_for_tmem((size_t)p.n_stages * p.stage_bytes + fixed + 1024, p.tmem_cols);
     static bool configured[64] = {};
     int dev = 0;
     B200Q_CUDA_TRY(cudaGetDevice(&dev));
@@ -237,16 +367,14 @@ static int launch_mx_gemm(const MxParams& p, int64_t x_tiles, size_t smem, cudaS
         B200Q_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    const int64_t blocks = x_tiles * p.row_tiles * p.split;
-    if (blocks > 2147483647LL) return fail(B200Q_ERR_UNSUPPORTED, "mx4: %lld blocks are more than a grid holds", (long long)blocks);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(kMxThreads);
+    cfg.gridDim = dim3((unsigned)(row_tiles * split), (unsigned)x_tiles);
+    cfg.blockDim = dim3(kMxThreads<XT>);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.split;
+    attr[0].val.clusterDim.x = (unsigned)split;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -257,27 +385,12 @@ static int launch_mx_gemm(const MxParams& p, int64_t x_tiles, size_t smem, cudaS
     return B200Q_OK;
 }
 
-int launch_mx4_wide(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
-                    int E, int sms, int* status, cudaStream_t st);
-
-static int g_mx4_wide = 1;
-void mx4_set_wide(int v) { g_mx4_wide = v; }
-int mx4_get_wide() { return g_mx4_wide; }
-static int g_mx4_few = 32;
-void mx4_set_few(int v) { g_mx4_few = v; }
-int mx4_get_few() { return g_mx4_few; }
-
-// One matrix (plan == nullptr: M rows of X) or the experts of a plan (buffer laid out for `pairs` pairs and E experts).
-int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K,
-                    const int* plan, int64_t pairs, int E, int sms, int* status, cudaStream_t st) {
-    const bool many = plan ? pairs >= 64LL * E : M >= 192;
-    if (g_mx4_wide == 2 || (g_mx4_wide == 1 && many))
-        return launch_mx4_wide(W, W_up, X, bias, bias_dtype, Y, y_dtype, M, N, K, plan, pairs, E, sms, status, st);
+static MxParams mx_params(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, const int* plan,
+                          int64_t pairs, int E, int* status, int64_t* x_tiles) {
     MxParams p = {};
-    const int mats = W_up ? 2 : 1;
     p.W = static_cast<const uint8_t*>(W);
     p.W_up = static_cast<const uint8_t*>(W_up);
-    p.X = static_cast<const uint8_t*>(X);
+    p.X = X;
     p.bias = bias;
     p.bias_dtype = bias_dtype;
     p.Y = Y;
@@ -287,38 +400,60 @@ int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* 
     p.N = N;
     p.K = K;
     p.k_tiles = mx_k_tiles(K);
-    p.row_tiles = (int)mx_row_tiles(N);
-    int64_t x_tiles = mx_row_tiles(M), rows_most = M;
+    p.pairs_per_row = 1;
+    p.experts = 1;
+    *x_tiles = mx_row_tiles(M);
     if (plan) {
         const MoePlanLayout l = moe_plan_layout(pairs, E);
         p.w_expert_bytes = mx_image_bytes(N, K);
         p.tiles = reinterpret_cast<const int4*>(plan + l.tiles);
         p.n_tiles = plan + l.n_tiles;
         p.order = plan + l.order;
-        x_tiles = l.max_tiles;
-        rows_most = pairs;
+        p.experts = E;
+        *x_tiles = l.max_tiles;
     }
-    p.n_cols = rows_most >= kMxTileRows ? kMxTileRows : (int)((rows_most + 15) & ~15);
-    p.stage_bytes = mats * kMxTileBytes + kMxSfBytes + p.n_cols * 128;
-    // Split K while the CTAs do not fill the SMs twice and every share keeps two tiles or more.
-    p.split = 1;
-    while (p.split < 8 && x_tiles * p.row_tiles * p.split * 2 <= 2 * sms && p.k_tiles >= 4 * p.split) p.split *= 2;
-    p.split_tiles = (p.k_tiles + p.split - 1) / p.split;
-    // Two CTAs share an SM where 256 TMEM columns do (accumulators and the stages' scales), else one has it alone. Shared memory is
-    // asked for such that TMEM cannot run out: CTAs that fit an SM by their shared memory fit its 512 columns too.
-    const int acc = mats * p.n_cols, sf = 8 * (mats + 1);
-    const bool two = acc + 4 * sf <= 256;
-    const int budget = two ? 110 * 1024 : 222 * 1024;
-    p.n_stages = budget / p.stage_bytes;
-    if (p.n_stages > kMxMaxStages) p.n_stages = kMxMaxStages;
-    const int cols = two ? 256 : 512;
-    while (acc + p.n_stages * sf > cols) --p.n_stages;
-    p.tmem_cols = (uint32_t)cols;
-    size_t smem = (size_t)p.n_stages * p.stage_bytes;
-    const size_t parts = p.split > 1 ? (size_t)mats * p.n_cols * 512 : 0;
-    if (smem < parts) smem = parts;
-    smem = mx_smem_for_tmem(smem + 1024, two ? 256 : 512);
-    return mats == 2 ? launch_mx_gemm<2>(p, x_tiles, smem, st) : launch_mx_gemm<1>(p, x_tiles, smem, st);
+    return p;
+}
+
+static int g_mx4_wide = 1, g_mx4_few = kMxDenseRows;
+void mx4_set_wide(int v) { g_mx4_wide = v; }
+int mx4_get_wide() { return g_mx4_wide; }
+void mx4_set_few(int v) { g_mx4_few = v; }
+int mx4_get_few() { return g_mx4_few; }
+
+int launch_mx4_wide(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
+                    int E, int early, int sms, int* status, cudaStream_t st);
+
+// X an image: M rows of one matrix (plan == nullptr), or the experts of a plan (buffer laid out for `pairs` pairs and E experts). `early`: the launch
+// before this one in the stream is the quantisation that made X.
+int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
+                    int E, int early, int sms, int* status, cudaStream_t st) {
+    const bool many = plan ? pairs >= 64LL * E : M >= 192;
+    if (g_mx4_wide == 2 || (g_mx4_wide == 1 && many))
+        return launch_mx4_wide(W, W_up, X, bias, bias_dtype, Y, y_dtype, M, N, K, plan, pairs, E, early, sms, status, st);
+    int64_t x_tiles;
+    MxParams p = mx_params(W, W_up, X, bias, bias_dtype, Y, y_dtype, M, N, K, plan, pairs, E, status, &x_tiles);
+    p.early = early && pdl_option() >= 0;
+    const int64_t rows_most = plan ? pairs : M;
+    return W_up ? launch_mx_gemm<2, void>(p, x_tiles, rows_most, sms, st) : launch_mx_gemm<1, void>(p, x_tiles, rows_most, sms, st);
+}
+
+// Whether a product of so many rows (of one matrix, or pairs of a plan: no group can be larger) runs as one launch on dense X.
+bool mx4_dense_takes(int64_t rows, int K) {
+    return rows <= (g_mx4_few < kMxDenseRows ? g_mx4_few : kMxDenseRows) && mx_k_tiles(K) <= 8 * kMxDenseTiles;
+}
+
+// X dense, of x_dtype (which the bias has too), for a product that mx4_dense_takes.
+int launch_mx4_dense(const void* W, const void* W_up, const void* X, int x_dtype, const void* bias, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
+                     int pairs_per_row, int E, int sms, int* status, cudaStream_t st) {
+    int64_t x_tiles;
+    MxParams p = mx_params(W, W_up, X, bias, x_dtype, Y, y_dtype, M, N, K, plan, pairs, E, status, &x_tiles);
+    p.pairs_per_row = pairs_per_row;
+    auto run = [&](auto zero) {
+        using XT = decltype(zero);
+        return W_up ? launch_mx_gemm<2, XT>(p, x_tiles, kMxDenseRows, sms, st) : launch_mx_gemm<1, XT>(p, x_tiles, kMxDenseRows, sms, st);
+    };
+    return x_dtype == B200Q_DT_F32 ? run(0.f) : x_dtype == B200Q_DT_F16 ? run(__half()) : run(__nv_bfloat16());
 }
 
 }  // namespace b200q

@@ -38,6 +38,7 @@ struct WideParams {
     int row_tiles;         // 128-row tiles of a weight matrix
     int w_tiles;           // 256-wide tiles of results: pairs of row tiles, or (gated) row tiles
     int bias_dtype, y_dtype;
+    int early;             // the predecessor writes neither weights nor plan (it is the quantisation): they are read ahead of its end
 };
 
 __device__ __forceinline__ void wide_alloc(uint32_t slot) {
@@ -111,11 +112,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
     __syncthreads();
     mx_cluster_sync();
     tc_fence_after();
-    grid_dep_wait();
+    if (!p.early || warp != 0) grid_dep_wait();
     const uint32_t tmem_base = tmem_base_slot;
 
     // A unit is two neighbouring activation tiles of one group (or its last one); an item is a unit x a 256-wide tile of weights.
-    const int units = p.units ? (int)ld_dep_u32(p.n_units) : (p.M + 2 * kMxTileRows - 1) / (2 * kMxTileRows);
+    const int units = p.units ? (int)ld_l2_u32(p.n_units) : (p.M + 2 * kMxTileRows - 1) / (2 * kMxTileRows);
     const int items = units * p.w_tiles;
     constexpr int kGroup = 8;  // units whose items are neighbours: the operands of concurrent tiles are shared in the L2
     struct Item {
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
         it.first = it.x_tile * kMxTileRows;
         it.rows = p.M - it.first;
         if (p.units) {
-            const uint4 u = ld_dep_u4(p.units + unit);
+            const uint4 u = ld_l2_u4(p.units + unit);
             it.expert = (int)u.x;
             it.first = (int)u.y + (int)crank * kMxTileRows;
             it.rows = (int)u.z - (int)crank * kMxTileRows;
@@ -161,29 +162,49 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
             const uint32_t x_bytes = (uint32_t)((it.rows + 7) & ~7) * 128u;
             // (a pair's second tile may lie behind the last: nothing of it is fetched, its rows of the accumulator are not used)
             const uint32_t bytes = (x_bytes ? x_bytes + kMxSfBytes : 0u) + kMxQBytes + 2 * kMxSfBytes;
-            for (int kt = 0; kt < p.k_tiles; ++kt) {
+            auto load_w = [&](int kt, uint32_t dst, uint32_t full) {
+                const size_t at = (size_t)kt * kMxTileBytes;
+                const uint32_t b = dst + kMxTileBytes;
+                mbar_arrive_expect_tx(full, bytes);
+                bulk_g2s(b, (crank ? w1 : w0) + at, kMxQBytes, full);
+                bulk_g2s(b + kMxQBytes, w0 + at + kMxQBytes, kMxSfBytes, full);
+                bulk_g2s(b + kMxQBytes + kMxSfBytes, w1 + at + kMxQBytes, kMxSfBytes, full);
+            };
+            auto load_x = [&](int kt, uint32_t dst, uint32_t full) {
+                const uint8_t* src = x + (size_t)kt * kMxTileBytes;
+                if (x_bytes == kMxQBytes) {
+                    bulk_g2s(dst, src, kMxTileBytes, full);
+                } else if (x_bytes) {
+                    bulk_g2s(dst, src, x_bytes, full);
+                    bulk_g2s(dst + kMxQBytes, src + kMxQBytes, kMxSfBytes, full);
+                }
+            };
+            int kt = 0;
+            if (i == worker) {  // the first stages' weights, then - behind the predecessor, whose results they are - the activations
+                const int head = min(p.k_tiles, kWideStages);
+                if (mx_elect())
+                    for (int s = 0; s < head; ++s) load_w(s, sbase + s * kWideStageBytes, smem_u32(&bar_full[s]));
+                __syncwarp();
+                if (p.early) grid_dep_wait();
+                if (mx_elect())
+                    for (int s = 0; s < head; ++s) load_x(s, sbase + s * kWideStageBytes, smem_u32(&bar_full[s]));
+                __syncwarp();
+                issued = kt = head;
+                slot = head == kWideStages ? 0 : head;
+                if (slot == 0) phase ^= 1;
+            }
+            for (; kt < p.k_tiles; ++kt) {
                 if (!(ok = mx_warp_wait(smem_u32(&bar_empty[slot]), phase, &abort_flag, p.status, kDevTimeoutEmpty))) break;
-                const uint32_t full = smem_u32(&bar_full[slot]), dst = sbase + slot * kWideStageBytes, b = dst + kMxTileBytes;
                 if (mx_elect()) {
-                    mbar_arrive_expect_tx(full, bytes);
-                    if (x_bytes == kMxQBytes) {
-                        bulk_g2s(dst, x, kMxTileBytes, full);
-                    } else if (x_bytes) {
-                        bulk_g2s(dst, x, x_bytes, full);
-                        bulk_g2s(dst + kMxQBytes, x + kMxQBytes, kMxSfBytes, full);
-                    }
-                    bulk_g2s(b, crank ? w1 : w0, kMxQBytes, full);
-                    bulk_g2s(b + kMxQBytes, w0 + kMxQBytes, kMxSfBytes, full);
-                    bulk_g2s(b + kMxQBytes + kMxSfBytes, w1 + kMxQBytes, kMxSfBytes, full);
+                    load_w(kt, sbase + slot * kWideStageBytes, smem_u32(&bar_full[slot]));
+                    load_x(kt, sbase + slot * kWideStageBytes, smem_u32(&bar_full[slot]));
                 }
                 __syncwarp();
-                x += kMxTileBytes;
-                w0 += kMxTileBytes;
-                w1 += kMxTileBytes;
                 ++issued;
                 if (++slot == kWideStages) { slot = 0; phase ^= 1; }
             }
         }
+        if (p.early && worker >= items) grid_dep_wait();
     } else if (warp == 2) {
         if (crank == 1) {
             int slot = 0;
@@ -325,8 +346,9 @@ static int launch_wide(const WideParams& p, int64_t units, int sms, cudaStream_t
 
 // One matrix (plan == nullptr: M rows of X) or the experts of a plan (buffer laid out for `pairs` pairs and E experts).
 int launch_mx4_wide(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
-                    int E, int sms, int* status, cudaStream_t st) {
+                    int E, int early, int sms, int* status, cudaStream_t st) {
     WideParams p = {};
+    p.early = early && pdl_option() >= 0;
     p.W = static_cast<const uint8_t*>(W);
     p.W_up = static_cast<const uint8_t*>(W_up);
     p.X = static_cast<const uint8_t*>(X);

@@ -276,8 +276,9 @@ int b200q_linear(int fmt, const void* W, const void* X, int x_dtype, const void*
  * b200q_mx4_gemm       Y(M,N) = X(M,K) W(N,K)^T (+ bias(N)) of two images: exact products, FP32 sums on the tensor cores, one rounding to
  *                      y_dtype. Any M >= 0; few output tiles have K split over a cluster's CTAs, with a fixed order of the sums: the
  *                      result does not change from run to run.
- * b200q_mx4_linear     the same from X of x_dtype, quantised into `ws` (b200q_mx4_linear_workspace_bytes(M, K) bytes, 256-byte aligned; a
- *                      larger one will do) on the way; bias is of x_dtype. Calls that share a workspace must be ordered on one stream.
+ * b200q_mx4_linear     the same from X of x_dtype, quantised on the way - up to 16 rows inside the product's launch, more into `ws`
+ *                      (b200q_mx4_linear_workspace_bytes(M, K) bytes, 256-byte aligned; a larger one will do, NULL where the size is 0); bias is of
+ *                      x_dtype. Calls that share a workspace must be ordered on one stream.
  */
 size_t b200q_mx4_image_bytes(int64_t rows, int K); /* 0 if K is not a positive multiple of 32 */
 int b200q_mx4_pack(const void* blocks, int64_t count, int64_t rows, int K, void* image, void* stream);
@@ -303,8 +304,8 @@ int b200q_mx4_linear(const void* W, const void* X, int x_dtype, const void* bias
  * b200q_moe_mx4_linear Y(pair, N) = quantise(X row) W_e(N,K)^T (+ bias_e(N)), e the pair's expert. W: E images of N x K, one
  *                      after the other (b200q_mx4_pack with count = E); X: tokens x K, a row for all pairs of its token, or with x_per_pair
  *                      tokens * k x K; bias: E x N of x_dtype or NULL; Y: tokens * k rows of N. Rows of pairs without an expert
- *                      are left as they were. `plan` must be of the same tokens, k and E. `ws`: b200q_moe_mx4_workspace_bytes() bytes,
- *                      256-byte aligned, shared only by calls that are ordered on one stream.
+ *                      are left as they were. `plan` must be of the same tokens, k and E. `ws`: b200q_moe_mx4_workspace_bytes() bytes
+ *                      (none for up to 16 pairs), 256-byte aligned, shared only by calls that are ordered on one stream.
  * b200q_moe_mx4_swiglu Y(pair, N) = silu(gate) * up of two such products, silu(v) = v / (1 + exp(-v)), without writing them out.
  * b200q_moe_combine    out(t, N) = sum over j of weights[t][j] * y(t, j, N), in the order of j in FP32; y and out of dtype. Pairs whose id
  *                      is outside 0 .. E - 1 are not read.
@@ -373,6 +374,8 @@ int b200q_device_status(int* status_out);
  *   "gemv_lean"   0 = never take the trimmed instantiation of the integer-dot kernel (FP32 in and out, no bias)
  *   "mx4_wide"    products of MXFP4 images: 1 (default) = the kernel of 256-wide tiles where there are many activation rows, 2 = for
  *                 every call, 0 = never
+ *   "mx4_few"     most rows (of a plan: pairs) of dense activations that the product's launch quantises itself: 0 .. 16 (default); the
+ *                 workspace sizes go by it
  *   "wait_limit_us" bound of the decode kernels' device-side waits (stage barriers, peer arrival) in
  *                 microseconds; 0 = one second. Tests shorten it to see a wait run out.
  *   "last_kernel" (read only) the kernel of the calling thread's last linear call, its last pass: 1 plain-load GEMV, 2 warp-MMA

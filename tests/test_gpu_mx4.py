@@ -92,10 +92,10 @@ def test_pack_takes_blocks_from_any_byte():
 
 @pytest.fixture(params=["as routed", "small tiles", "wide tiles", "few rows"])
 def route(request):
-    """Each kernel takes every call (that of few rows, every call of up to 32 of them) and is held to the definition whatever the routing rules say."""
+    """Each kernel takes every call (that of few rows, every call of up to 16 of them) and is held to the definition whatever the routing rules say."""
     was = ops.get_option("mx4_wide"), ops.get_option("mx4_few")
     ops.set_option("mx4_wide", {"small tiles": 0, "wide tiles": 2}.get(request.param, was[0]))
-    ops.set_option("mx4_few", {"small tiles": 0, "wide tiles": 0, "few rows": 32}.get(request.param, was[1]))
+    ops.set_option("mx4_few", {"small tiles": 0, "wide tiles": 0, "few rows": 16}.get(request.param, was[1]))
     yield
     ops.set_option("mx4_wide", was[0])
     ops.set_option("mx4_few", was[1])

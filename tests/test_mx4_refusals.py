@@ -30,9 +30,13 @@ def test_sizes(L):
     assert L.b200q_mx4_image_bytes(0, 64) == 0 and L.b200q_mx4_image_bytes(4, 48) == 0 and L.b200q_mx4_image_bytes(-1, 32) == 0
     assert L.b200q_mx4_image_bytes(2 ** 33, 4096) == 2 ** 33 // 128 * 16 * 17408
     assert L.b200q_mx4_linear_workspace_bytes(300, 1024) == L.b200q_mx4_image_bytes(300, 1024)
-    # tiles of 128 pairs: one pair, one tile; eight pairs at most eight; never more than pairs / 128 and one for each expert
-    assert L.b200q_moe_mx4_workspace_bytes(1, 1, 64, 256) == 17408
-    assert L.b200q_moe_mx4_workspace_bytes(1, 8, 64, 256) == 8 * 17408
+    # up to 16 rows are quantised inside the product's launch, unless they are very long
+    assert L.b200q_mx4_linear_workspace_bytes(16, 65536) == 0 and L.b200q_mx4_linear_workspace_bytes(17, 256) == 17408
+    assert L.b200q_mx4_linear_workspace_bytes(1, 1 << 20) == L.b200q_mx4_image_bytes(1, 1 << 20)
+    assert L.b200q_moe_mx4_workspace_bytes(2, 8, 64, 4096) == 0
+    # tiles of 128 pairs: seventeen pairs at most seventeen; never more than pairs / 128 and one for each expert
+    assert L.b200q_moe_mx4_workspace_bytes(17, 1, 64, 256) == 17 * 17408
+    assert L.b200q_moe_mx4_workspace_bytes(3, 8, 4, 256) == 4 * 17408
     assert L.b200q_moe_mx4_workspace_bytes(512, 8, 64, 256) == (32 + 64) * 17408
     for t, k, e in ((-1, 1, 1), (1, 0, 4), (1, 33, 64), (1, 1, 0), (1, 1, 1025)):
         assert L.b200q_moe_plan_bytes(t, k, e) == 0 and L.b200q_moe_mx4_workspace_bytes(t, k, e, 256) == 0
@@ -42,7 +46,9 @@ def test_sizes(L):
 @pytest.mark.parametrize("pairs,E", [(1, 1), (5, 3), (128, 1), (129, 1), (130, 2), (1000, 7), (256, 300)])
 def test_the_tiles_of_any_grouping_fit(L, pairs, E):
     """Every way to cut the groups that can need many tiles: one large group and single pairs, or groups of 128 i + 1."""
+    L.b200q_set_option(b"mx4_few", 0)
     most = L.b200q_moe_mx4_workspace_bytes(pairs, 1, E, 256) // 17408
+    L.b200q_set_option(b"mx4_few", 16)
     for met in range(1, min(E, pairs) + 1):
         sizes = [1] * (met - 1)
         left = pairs - (met - 1)
@@ -68,7 +74,7 @@ def test_mx4_arguments(L, p):
     assert g(W=None) == BAD and g(X=p + 8) == BAD and g(Y=p + 2) == BAD and g(yt=3) == BAD and g(bt=7) == BAD
     assert g(b=p + 1, bt=capi.F16) == BAD and g(M=-1) == BAD and g(N=-1) == BAD and g(K=16) == BAD
     assert g(M=0) == OK and g(N=0) == OK
-    lin = lambda X=p, ws=p, n=1 << 20, M=1, K=32, xt=f32: L.b200q_mx4_linear(p, X, xt, None, p, f32, M, 4, K, ws, n, None)
+    lin = lambda X=p, ws=p, n=1 << 20, M=20, K=32, xt=f32: L.b200q_mx4_linear(p, X, xt, None, p, f32, M, 4, K, ws, n, None)
     assert lin(ws=None) == WS and lin(n=17407) == WS and lin(ws=p + 16) == WS and b"17408 bytes" in L.b200q_last_error()
     assert lin(X=p + 4) == BAD and lin(X=None) == BAD and lin(xt=5) == BAD and lin(K=8) == BAD and lin(M=-3) == BAD and lin(M=0, ws=None) == OK
 
@@ -83,7 +89,7 @@ def test_moe_arguments(L, p):
     assert r(k=9) == BAD and b"more than E" in L.b200q_last_error()
     assert r(dt=3) == BAD and r(lg=None) == BAD and r(ids=None) == BAD and r(w=None) == BAD and r(lg=p + 2) == BAD and r(plan=p + 8) == BAD
     assert r(T=0, plan=None, lg=None) == OK
-    m = lambda W=p, X=p, xt=f32, plan=p, b=None, Y=p, yt=f32, T=2, k=2, E=4, N=8, K=32, ws=p, n=1 << 30: L.b200q_moe_mx4_linear(
+    m = lambda W=p, X=p, xt=f32, plan=p, b=None, Y=p, yt=f32, T=20, k=2, E=4, N=8, K=32, ws=p, n=1 << 30: L.b200q_moe_mx4_linear(
         W, X, xt, 0, plan, b, Y, yt, T, k, E, N, K, ws, n, None)
     assert m(W=None) == BAD and m(X=None) == BAD and m(plan=None) == BAD and m(Y=None) == BAD and m(xt=3) == BAD and m(yt=3) == BAD
     assert m(W=p + 8) == BAD and m(X=p + 8) == BAD and m(plan=p + 4) == BAD and m(Y=p + 1) == BAD and m(b=p + 2) == BAD
