@@ -13,8 +13,8 @@ int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* 
 int launch_mx4_dense(const void* W, const void* W_up, const void* X, int x_dtype, const void* bias, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
                    int pairs_per_row, int E, int sms, int* status, cudaStream_t st);
 bool mx4_dense_takes(int64_t rows, int K);
-int launch_moe_topk(const void* logits, int dtype, int64_t tokens, int E, int k, int normalize, float scale, int* ids, float* weights, int sms, cudaStream_t st);
-int launch_moe_plan(const int* ids, int64_t pairs, int E, int* plan, cudaStream_t st);
+int launch_moe_route(const void* logits, int dtype, int64_t tokens, int E, int k, int normalize, float scale, int* ids, float* weights, int* plan, cudaStream_t st);
+int launch_moe_plan(const int* ids, int64_t tokens, int k, int E, int* plan, cudaStream_t st);
 int launch_moe_combine(const void* y, int dtype, const int* ids, const float* weights, int64_t tokens, int k, int N, int E, void* out, int sms, cudaStream_t st);
 
 static bool dtype_ok(int dt) { return dt == B200Q_DT_F32 || dt == B200Q_DT_F16 || dt == B200Q_DT_BF16; }
@@ -130,7 +130,7 @@ int b200q_moe_plan(const int32_t* ids, int64_t tokens, int k, int E, void* plan,
     if (!on(ids, 4) || !on(plan, 16)) return fail(B200Q_ERR_BAD_ARG, "moe_plan: ids must be 4-byte and the plan 16-byte aligned");
     int sms, *status;
     if (int rc = device_facts(&sms, &status)) return rc;
-    return launch_moe_plan(ids, tokens * k, E, static_cast<int*>(plan), static_cast<cudaStream_t>(stream));
+    return launch_moe_plan(ids, tokens, k, E, static_cast<int*>(plan), static_cast<cudaStream_t>(stream));
 }
 
 int b200q_moe_route(const void* logits, int dtype, int64_t tokens, int E, int k, int normalize, float scale, int32_t* ids, float* weights, void* plan, void* stream) {
@@ -143,10 +143,7 @@ int b200q_moe_route(const void* logits, int dtype, int64_t tokens, int E, int k,
     if (tokens == 0 && !plan) return B200Q_OK;
     int sms, *status;
     if (int rc = device_facts(&sms, &status)) return rc;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (tokens)
-        if (int rc = launch_moe_topk(logits, dtype, tokens, E, k, normalize, scale, ids, weights, sms, st)) return rc;
-    return plan ? launch_moe_plan(ids, tokens * k, E, static_cast<int*>(plan), st) : B200Q_OK;
+    return launch_moe_route(logits, dtype, tokens, E, k, normalize, scale, ids, weights, static_cast<int*>(plan), static_cast<cudaStream_t>(stream));
 }
 
 size_t b200q_moe_mx4_workspace_bytes(int64_t tokens, int k, int E, int K) {

@@ -29,13 +29,12 @@ inline __host__ __device__ size_t mx_image_bytes(int64_t rows, int K) { return (
 // their order; it is cut into tiles of 128, the row tiles of the activation image.
 //   offsets[E + 1] | order[pairs] (pairs by expert, -1 behind the last) | place[pairs] (tile * 128 + row of pair s, or -1) |
 //   n_tiles, n_units, 2 unused | tiles[max_tiles] {expert, first place in `order`, pairs, 0}, 16-byte aligned |
-//   units[max_units], two neighbouring tiles of an expert or its last one: {expert, first place, pairs, tile} | counts of the blocks
+//   units[max_units], two neighbouring tiles of an expert or its last one: {expert, first place, pairs, tile} | counts of the ranges
 struct MoePlanLayout {
     size_t order, place, n_tiles, tiles, units, hist, total;
     int64_t max_tiles, max_units;
-    int hist_blocks;
 };
-constexpr int kPlanBlockPairs = 1024;
+constexpr int kPlanRanges = 128;  // ranges of tokens that the grouping counts apart
 inline __host__ MoePlanLayout moe_plan_layout(int64_t pairs, int E) {
     MoePlanLayout l;
     const int64_t met = pairs < E ? pairs : E;
@@ -43,14 +42,13 @@ inline __host__ MoePlanLayout moe_plan_layout(int64_t pairs, int E) {
     if (l.max_tiles > pairs) l.max_tiles = pairs;
     l.max_units = pairs / (2 * kMxTileRows) + met;
     if (l.max_units > pairs) l.max_units = pairs;
-    l.hist_blocks = (int)((pairs + kPlanBlockPairs - 1) / kPlanBlockPairs);
     l.order = (size_t)E + 1;
     l.place = l.order + (size_t)pairs;
     l.n_tiles = (l.place + (size_t)pairs + 3) & ~(size_t)3;
     l.tiles = l.n_tiles + 4;
     l.units = l.tiles + 4 * (size_t)l.max_tiles;
     l.hist = l.units + 4 * (size_t)l.max_units;
-    l.total = l.hist + (size_t)l.hist_blocks * (size_t)E;
+    l.total = l.hist + (size_t)kPlanRanges * (size_t)E;
     return l;
 }
 

@@ -428,7 +428,11 @@ int launch_mx4_wide(const void* W, const void* W_up, const void* X, const void* 
 // before this one in the stream is the quantisation that made X.
 int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
                     int E, int early, int sms, int* status, cudaStream_t st) {
-    const bool many = plan ? pairs >= 64LL * E : M >= 192;
+    // Where the wide tiles are the faster ones, by measurement (small tiles' time grows with the rows, the wide ones' hardly; us, small and wide):
+    // 14336 x 4096 at 32 / 48 / 64 rows 12.7 13.4 / 14.9 13.6 / 17.0 13.7 - row tiles for every SM, nothing to split -, 4096 x 4096 at 64 / 96 / 128
+    // 9.5 11.8 / 11.8 12.0 / 28.0 12.0, 1024 x 4096 at 64 / 128 / 256 7.1 10.9 / 10.4 11.3 / 18.5 11.5. Experts, on average 8 / 16 / 32 pairs each:
+    // 128 gated 768 x 2048 41.5 38.8 (8) / 50.2 42.4 / 58.4 45.7, 32 of 2048 x 2048 16.9 18.7 / 18.6 18.9 / 27.2 20.9, 8 gated 4096 x 4096 30.1 30.7 / 31.7 30.6 / 36.6 32.0.
+    const bool many = plan ? pairs >= 16LL * E : M >= (mx_row_tiles(N) * 2 > sms ? 48 : 112);
     if (g_mx4_wide == 2 || (g_mx4_wide == 1 && many))
         return launch_mx4_wide(W, W_up, X, bias, bias_dtype, Y, y_dtype, M, N, K, plan, pairs, E, early, sms, status, st);
     int64_t x_tiles;

@@ -179,50 +179,62 @@ def linear(fmt, W, X, N, bias=None, out=None, out_dtype=None, ws=None):
 
 # ---- MXFP4 matrices and sparse expert layers on them -------------------------------------------------------
 
+# (The wrappers below are written for short calls: a decode step makes a dozen of them per layer, and at a few microseconds each every torch
+# call on the way counts.)
+
 def mx4_image_bytes(rows: int, K: int) -> int:
     """Bytes of the image of a rows x K matrix in MXFP4 (K a multiple of 32)."""
     if rows < 0 or K <= 0 or K % 32:
         raise ValueError(f"K ({K}) must be a positive multiple of 32")
-    return capi.lib().b200q_mx4_image_bytes(rows, K)
+    return ((rows + 127) >> 7) * ((K + 255) >> 8) * 17408
 
 
-def _check_image(W: torch.Tensor, rows: int, K: int, count: int = 1) -> None:
-    if W.dtype != torch.uint8 or not W.is_cuda or not W.is_contiguous():
+def _check_image(W: torch.Tensor, rows: int, K: int, count: int = 1) -> int:
+    """Returns the device index of an image that is one."""
+    device = W.get_device()
+    if device < 0 or W.dtype != torch.uint8 or not W.is_contiguous():
         raise ValueError("an image is a contiguous CUDA uint8 tensor (mx4_pack, mx4_quantize)")
-    need = count * mx4_image_bytes(rows, K)
-    if W.numel() < need:
-        raise ValueError(f"the image holds {W.numel()} bytes, {count} x ({rows}, {K}) needs {need}")
+    if W.numel() < count * mx4_image_bytes(rows, K):
+        raise ValueError(f"the image holds {W.numel()} bytes, {count} x ({rows}, {K}) needs {count * mx4_image_bytes(rows, K)}")
+    return device
 
 
-def _check_dense(t: torch.Tensor, what: str, device: torch.device) -> None:
-    if t.dtype not in _DT or not t.is_contiguous():
+def _check_dense(t: torch.Tensor, what: str, device: int) -> int:
+    """Returns the type code of a contiguous tensor of one of the dense types on device `device`."""
+    code = _DT.get(t.dtype)
+    if code is None or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous float32, float16 or bfloat16 tensor")
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, not on {device}")
+    if t.get_device() != device or device < 0:
+        raise ValueError(f"{what} is on {t.device}, not on CUDA device {device}")
+    return code
 
 
-def _check_int32(t: torch.Tensor, what: str, shape, device: torch.device) -> None:
-    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != tuple(shape):
+def _check_int32(t: torch.Tensor, what: str, shape, device: int) -> None:
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.shape != shape:
         raise ValueError(f"{what} must be a contiguous int32 tensor of shape {tuple(shape)}")
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, not on {device}")
+    if t.get_device() != device or device < 0:
+        raise ValueError(f"{what} is on {t.device}, not on CUDA device {device}")
 
 
-def _result(out, shape, out_dtype, x: torch.Tensor) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=out_dtype or (torch.float16 if x.dtype == torch.float16 else torch.float32), device=x.device)
-    if tuple(out.shape) != tuple(shape) or (out_dtype is not None and out.dtype != out_dtype):
+def _check_out(out: torch.Tensor, shape, out_dtype, device: int) -> None:
+    if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"out must be of shape {tuple(shape)}" + (f" and {out_dtype}" if out_dtype is not None else ""))
-    _check_dense(out, "out", x.device)
-    return out
+    _check_dense(out, "out", device)
 
 
-def _scratch(ws, need: int, device: torch.device) -> torch.Tensor:
+def _default_out(x: torch.Tensor) -> torch.dtype:
+    return torch.float16 if x.dtype == torch.float16 else torch.float32
+
+
+def _scratch(ws, need: int, x: torch.Tensor):
+    """(pointer, bytes) of the workspace, made here where the caller gives none; and the tensor, to be kept until the call is made."""
     if ws is None:
-        return torch.empty(need, dtype=torch.uint8, device=device)
-    if ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.device != device:
-        raise ValueError(f"ws must be a contiguous uint8 tensor on {device}")
-    return ws
+        if not need:
+            return None, 0, None
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    elif ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.device != x.device:
+        raise ValueError(f"ws must be a contiguous uint8 tensor on {x.device}")
+    return ws.data_ptr(), ws.numel(), ws
 
 
 def mx4_pack(blocks: torch.Tensor, rows: int, K: int, count: int = 1, out=None) -> torch.Tensor:
@@ -234,8 +246,8 @@ def mx4_pack(blocks: torch.Tensor, rows: int, K: int, count: int = 1, out=None) 
         raise ValueError(f"blocks hold {blocks.numel()} bytes, {count} x ({rows}, {K}) needs {count * rows * (K // 32) * 17}")
     if out is None:
         out = torch.empty(count * size, dtype=torch.uint8, device=blocks.device)
-    else:
-        _check_image(out, rows, K, count)
+    elif _check_image(out, rows, K, count) != blocks.get_device():
+        raise ValueError("out is on another device than the blocks")
     capi.check(_launch(blocks, capi.lib().b200q_mx4_pack, blocks.data_ptr(), count, rows, K, out.data_ptr()))
     return out
 
@@ -244,43 +256,45 @@ def mx4_quantize(x: torch.Tensor, out=None) -> torch.Tensor:
     """(rows, K) float32 / float16 / bfloat16 -> image."""
     if x.dim() != 2:
         raise ValueError("x must be (rows, K)")
-    _check_dense(x, "x", x.device)
+    device = x.get_device()
+    code = _check_dense(x, "x", device)
     rows, K = x.shape
     size = mx4_image_bytes(rows, K)
     if out is None:
         out = torch.empty(size, dtype=torch.uint8, device=x.device)
-    else:
-        _check_image(out, rows, K)
-    capi.check(_launch(x, capi.lib().b200q_mx4_quantize, x.data_ptr(), _DT[x.dtype], rows, K, out.data_ptr()))
+    elif _check_image(out, rows, K) != device:
+        raise ValueError("out is on another device than x")
+    capi.check(_launch(x, capi.lib().b200q_mx4_quantize, x.data_ptr(), code, rows, K, out.data_ptr()))
     return out
 
 
 def mx4_dequantize(image: torch.Tensor, rows: int, K: int, out_dtype=torch.float32) -> torch.Tensor:
     """The values of an image, (rows, K)."""
     _check_image(image, rows, K)
-    out = torch.empty((rows, K), dtype=out_dtype, device=image.device)
-    capi.check(_launch(image, capi.lib().b200q_mx4_dequantize, image.data_ptr(), rows, K, out.data_ptr(), _DT[out_dtype]))
+    code = _DT.get(out_dtype)
+    if code is None:
+        raise ValueError("out_dtype must be float32, float16 or bfloat16")
+    out = torch.empty(rows, K, dtype=out_dtype, device=image.device)
+    capi.check(_launch(image, capi.lib().b200q_mx4_dequantize, image.data_ptr(), rows, K, out.data_ptr(), code))
     return out
 
 
-def mx4_gemm(W: torch.Tensor, X: torch.Tensor, M: int, N: int, K: int, bias=None, out=None, out_dtype=torch.float32) -> torch.Tensor:
-    """Y(M,N) = X(M,K) @ W(N,K).T (+bias) of two images."""
-    _check_image(W, N, K)
-    _check_image(X, M, K)
-    if X.device != W.device:
+def mx4_gemm(W: torch.Tensor, X: torch.Tensor, M: int, N: int, K: int, bias=None, out=None, out_dtype=None) -> torch.Tensor:
+    """Y(M,N) = X(M,K) @ W(N,K).T (+bias) of two images; float32 unless out_dtype says otherwise."""
+    device = _check_image(W, N, K)
+    if _check_image(X, M, K) != device:
         raise ValueError("W and X are on different devices")
+    bias_code = capi.F32
     if bias is not None:
-        _check_dense(bias, "bias", W.device)
+        bias_code = _check_dense(bias, "bias", device)
         if bias.numel() != N:
             raise ValueError("bias must have N elements")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=W.device)
+        out = torch.empty(M, N, dtype=out_dtype or torch.float32, device=W.device)
     else:
-        _check_dense(out, "out", W.device)
-        if tuple(out.shape) != (M, N):
-            raise ValueError(f"out must be of shape {(M, N)}")
-    capi.check(_launch(W, capi.lib().b200q_mx4_gemm, W.data_ptr(), X.data_ptr(), bias.data_ptr() if bias is not None else None,
-                       _DT[bias.dtype] if bias is not None else capi.F32, out.data_ptr(), _DT[out.dtype], M, N, K))
+        _check_out(out, (M, N), out_dtype, device)
+    capi.check(_launch(W, capi.lib().b200q_mx4_gemm, W.data_ptr(), X.data_ptr(), bias.data_ptr() if bias is not None else None, bias_code,
+                       out.data_ptr(), _DT[out.dtype], M, N, K))
     return out
 
 
@@ -291,17 +305,20 @@ def mx4_linear(W: torch.Tensor, X: torch.Tensor, N: int, bias=None, out=None, ou
     if X.dim() != 2:
         raise ValueError("X must be (M, K)")
     M, K = X.shape
-    _check_image(W, N, K)
-    _check_dense(X, "X", W.device)
+    device = _check_image(W, N, K)
+    code = _check_dense(X, "X", device)
+    bias_ptr = None
     if bias is not None:
-        _check_dense(bias, "bias", X.device)
-        if bias.dtype != X.dtype or bias.numel() != N:
+        if _check_dense(bias, "bias", device) != code or bias.numel() != N:
             raise ValueError("bias must have N elements of X's dtype")
-    out = _result(out, (M, N), out_dtype, X)
+        bias_ptr = bias.data_ptr()
+    if out is None:
+        out = torch.empty(M, N, dtype=out_dtype or _default_out(X), device=X.device)
+    else:
+        _check_out(out, (M, N), out_dtype, device)
     L = capi.lib()
-    ws = _scratch(ws, L.b200q_mx4_linear_workspace_bytes(M, K), X.device)
-    capi.check(_launch(X, L.b200q_mx4_linear, W.data_ptr(), X.data_ptr(), _DT[X.dtype], bias.data_ptr() if bias is not None else None,
-                       out.data_ptr(), _DT[out.dtype], M, N, K, ws.data_ptr(), ws.numel()))
+    ws_ptr, ws_bytes, ws = _scratch(ws, L.b200q_mx4_linear_workspace_bytes(M, K), X)
+    capi.check(_launch(X, L.b200q_mx4_linear, W.data_ptr(), X.data_ptr(), code, bias_ptr, out.data_ptr(), _DT[out.dtype], M, N, K, ws_ptr, ws_bytes))
     return out
 
 
@@ -309,12 +326,14 @@ class MoePlan:
     """The pairs of tokens and experts grouped by expert. offsets (E + 1) and order (tokens * k): expert e has the pairs
     order[offsets[e]:offsets[e + 1]], in their own order; pair s = t * k + j is token t's j-th choice. Device tensors, int32."""
 
+    __slots__ = ("tokens", "k", "experts", "data")
+
     def __init__(self, tokens: int, k: int, experts: int, device):
         size = capi.lib().b200q_moe_plan_bytes(tokens, k, experts)
         if not size:
             raise ValueError(f"{tokens} tokens, {k} of {experts} experts each: outside the supported sizes (1..1024 experts, 1..32 each)")
         self.tokens, self.k, self.experts = tokens, k, experts
-        self.data = torch.empty(size // 4, dtype=torch.int32, device=device)
+        self.data = torch.empty(size >> 2, dtype=torch.int32, device=device)
 
     @property
     def offsets(self) -> torch.Tensor:
@@ -327,9 +346,9 @@ class MoePlan:
 
 def moe_plan(ids: torch.Tensor, experts: int) -> MoePlan:
     """Groups (tokens, k) int32 expert ids by expert. An id outside 0 .. experts - 1 is no expert."""
-    if ids.dim() != 2 or not ids.is_cuda:
+    if ids.dim() != 2:
         raise ValueError("ids must be a (tokens, k) CUDA tensor")
-    _check_int32(ids, "ids", ids.shape, ids.device)
+    _check_int32(ids, "ids", ids.shape, ids.get_device())
     plan = MoePlan(ids.shape[0], ids.shape[1], experts, ids.device)
     capi.check(_launch(ids, capi.lib().b200q_moe_plan, ids.data_ptr(), plan.tokens, plan.k, experts, plan.data.data_ptr()))
     return plan
@@ -338,69 +357,74 @@ def moe_plan(ids: torch.Tensor, experts: int) -> MoePlan:
 def moe_route(logits: torch.Tensor, k: int, normalize: bool = True, scale: float = 1.0):
     """(tokens, E) logits -> (ids, weights, plan): the k best experts of each token, ties to the lower one; their softmax
     weights over the chosen (normalize) or over all experts, times scale; the grouping by expert."""
-    if logits.dim() != 2 or not logits.is_cuda:
+    if logits.dim() != 2:
         raise ValueError("logits must be a (tokens, E) CUDA tensor")
-    _check_dense(logits, "logits", logits.device)
+    code = _check_dense(logits, "logits", logits.get_device())
     T, E = logits.shape
-    plan = MoePlan(T, k, E, logits.device)
-    ids = torch.empty((T, k), dtype=torch.int32, device=logits.device)
-    weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
-    capi.check(_launch(logits, capi.lib().b200q_moe_route, logits.data_ptr(), _DT[logits.dtype], T, E, k, int(normalize), float(scale),
-                       ids.data_ptr(), weights.data_ptr(), plan.data.data_ptr()))
+    device = logits.device
+    plan = MoePlan(T, k, E, device)
+    ids = torch.empty(T, k, dtype=torch.int32, device=device)
+    weights = torch.empty(T, k, dtype=torch.float32, device=device)
+    capi.check(_launch(logits, capi.lib().b200q_moe_route, logits.data_ptr(), code, T, E, k, 1 if normalize else 0, scale, ids.data_ptr(),
+                       weights.data_ptr(), plan.data.data_ptr()))
     return ids, weights, plan
 
 
-def _moe_mx4(entry, Ws, X, plan, N, bias, out, out_dtype, ws):
+def _moe_common(Ws, X, plan, N, out, out_dtype, ws):
+    """Checks; returns (type code of X, 1 if X has a row per pair, out, K, workspace)."""
     T, k, E = plan.tokens, plan.k, plan.experts
-    per_pair = X.dim() == 3
-    if X.dim() not in (2, 3) or X.shape[0] != T or (per_pair and X.shape[1] != k):
+    shape = X.shape
+    if (len(shape) != 2 and (len(shape) != 3 or shape[1] != k)) or shape[0] != T:
         raise ValueError(f"X must be ({T}, K) or ({T}, {k}, K), as the plan")
-    K = X.shape[-1]
-    _check_dense(X, "X", plan.data.device)
+    device, K = plan.data.get_device(), shape[-1]
+    code = _check_dense(X, "X", device)
     for W in Ws:
-        _check_image(W, N, K, E)
-        if W.device != X.device:
+        if _check_image(W, N, K, E) != device:
             raise ValueError("the weights are on another device than X")
-    if bias is not None:
-        _check_dense(bias, "bias", X.device)
-        if bias.dtype != X.dtype or tuple(bias.shape) != (E, N):
-            raise ValueError("bias must be (experts, N) of X's dtype")
-    out = _result(out, (T, k, N), out_dtype, X)
-    L = capi.lib()
-    ws = _scratch(ws, L.b200q_moe_mx4_workspace_bytes(T, k, E, K), X.device)
-    head = [W.data_ptr() for W in Ws] + [X.data_ptr(), _DT[X.dtype], int(per_pair), plan.data.data_ptr()]
-    if len(Ws) == 1:
-        head.append(bias.data_ptr() if bias is not None else None)
-    capi.check(_launch(X, entry(L), *head, out.data_ptr(), _DT[out.dtype], T, k, E, N, K, ws.data_ptr(), ws.numel()))
-    return out
+    if out is None:
+        out = torch.empty(T, k, N, dtype=out_dtype or _default_out(X), device=X.device)
+    else:
+        _check_out(out, (T, k, N), out_dtype, device)
+    return code, len(shape) - 2, out, K, _scratch(ws, capi.lib().b200q_moe_mx4_workspace_bytes(T, k, E, K), X)
 
 
 def moe_mx4_linear(W, X, plan: MoePlan, N: int, bias=None, out=None, out_dtype=None, ws=None) -> torch.Tensor:
     """out[t][j] = quantise(X[t] or X[t][j]) @ W[e].T (+ bias[e]), e the j-th expert of token t: (tokens, k, N). W: the
     experts' images, one after the other. Rows of pairs without an expert are left as they were."""
-    return _moe_mx4(lambda L: L.b200q_moe_mx4_linear, [W], X, plan, N, bias, out, out_dtype, ws)
+    code, per_pair, out, K, (ws_ptr, ws_bytes, ws) = _moe_common((W,), X, plan, N, out, out_dtype, ws)
+    bias_ptr = None
+    if bias is not None:
+        if _check_dense(bias, "bias", X.get_device()) != code or bias.shape != (plan.experts, N):
+            raise ValueError("bias must be (experts, N) of X's dtype")
+        bias_ptr = bias.data_ptr()
+    capi.check(_launch(X, capi.lib().b200q_moe_mx4_linear, W.data_ptr(), X.data_ptr(), code, per_pair, plan.data.data_ptr(), bias_ptr, out.data_ptr(),
+                       _DT[out.dtype], plan.tokens, plan.k, plan.experts, N, K, ws_ptr, ws_bytes))
+    return out
 
 
 def moe_mx4_swiglu(W_gate, W_up, X, plan: MoePlan, N: int, out=None, out_dtype=None, ws=None) -> torch.Tensor:
-    """silu(gate) * up of the two products, in one launch behind the quantisation."""
-    return _moe_mx4(lambda L: L.b200q_moe_mx4_swiglu, [W_gate, W_up], X, plan, N, None, out, out_dtype, ws)
+    """silu(gate) * up of the two products, without writing them out."""
+    code, per_pair, out, K, (ws_ptr, ws_bytes, ws) = _moe_common((W_gate, W_up), X, plan, N, out, out_dtype, ws)
+    capi.check(_launch(X, capi.lib().b200q_moe_mx4_swiglu, W_gate.data_ptr(), W_up.data_ptr(), X.data_ptr(), code, per_pair, plan.data.data_ptr(),
+                       out.data_ptr(), _DT[out.dtype], plan.tokens, plan.k, plan.experts, N, K, ws_ptr, ws_bytes))
+    return out
 
 
-def moe_combine(y: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, experts: int | None = None, out=None) -> torch.Tensor:
+def moe_combine(y: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, experts: int = 2 ** 31 - 1, out=None) -> torch.Tensor:
     """out[t] = sum_j weights[t][j] * y[t][j]; pairs whose id is negative (or not below `experts`) are left out."""
-    if y.dim() != 3 or not y.is_cuda:
+    if y.dim() != 3:
         raise ValueError("y must be a (tokens, k, N) CUDA tensor")
-    _check_dense(y, "y", y.device)
     T, k, N = y.shape
-    _check_int32(ids, "ids", (T, k), y.device)
-    if weights.dtype != torch.float32 or not weights.is_contiguous() or tuple(weights.shape) != (T, k) or weights.device != y.device:
+    device = y.get_device()
+    code = _check_dense(y, "y", device)
+    _check_int32(ids, "ids", (T, k), device)
+    if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.shape != (T, k) or weights.get_device() != device:
         raise ValueError(f"weights must be a contiguous float32 tensor of shape {(T, k)} on {y.device}")
     if out is None:
-        out = torch.empty((T, N), dtype=y.dtype, device=y.device)
+        out = torch.empty(T, N, dtype=y.dtype, device=y.device)
     else:
-        out = _result(out, (T, N), y.dtype, y)
-    capi.check(_launch(y, capi.lib().b200q_moe_combine, y.data_ptr(), _DT[y.dtype], ids.data_ptr(), weights.data_ptr(), T, k,
-                       experts if experts is not None else 2 ** 31 - 1, N, out.data_ptr()))
+        _check_out(out, (T, N), y.dtype, device)
+    capi.check(_launch(y, capi.lib().b200q_moe_combine, y.data_ptr(), code, ids.data_ptr(), weights.data_ptr(), T, k, experts, N, out.data_ptr()))
     return out
 
 
