@@ -203,8 +203,16 @@ __device__ __forceinline__ void route_place(const RouteParams& p, int64_t s0, in
             tile0[e] = at[1];
             if (range == 0) {
                 p.offsets[e] = at[0];
-                for (int x = 0; x < t; ++x) p.tiles[at[1] + x] = make_int4(e, at[0] + x * kMxTileRows, min(kMxTileRows, n - x * kMxTileRows), 0);
-                for (int x = 0; x < u; ++x) p.units[at[2] + x] = make_int4(e, at[0] + x * 2 * kMxTileRows, min(2 * kMxTileRows, n - x * 2 * kMxTileRows), at[1] + 2 * x);
+                for (int x = 0; x < t; ++x) {  // (the fourth word comes from the block that places the tile's first pair)
+                    int4* tile = p.tiles + at[1] + x;
+                    tile->x = e;
+                    tile->y = at[0] + x * kMxTileRows;
+                    tile->z = min(kMxTileRows, n - x * kMxTileRows);
+                }
+                for (int x = 0; x < u; ++x) {
+                    p.units[2 * (at[2] + x)] = make_int4(e, at[0] + x * 2 * kMxTileRows, min(2 * kMxTileRows, n - x * 2 * kMxTileRows), at[1] + 2 * x);
+                    p.units[2 * (at[2] + x) + 1] = make_int4(at[2], u, 0, 0);
+                }
             }
         }
         at[0] += n;
@@ -245,6 +253,7 @@ __device__ __forceinline__ void route_place(const RouteParams& p, int64_t s0, in
                 const int place = next[e] - before[kWarps * E + e] + before[warp * E + e] + rank, i = place - first[e];
                 p.order[place] = (int)s;
                 p.place[s] = (tile0[e] + (i >> 7)) * kMxTileRows + (i & 127);
+                if ((i & 127) == 0) p.tiles[tile0[e] + (i >> 7)].w = (int)s;
             } else {
                 p.place[s] = -1;
             }

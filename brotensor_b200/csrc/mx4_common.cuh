@@ -28,8 +28,9 @@ inline __host__ __device__ size_t mx_image_bytes(int64_t rows, int K) { return (
 // The grouping of token-expert pairs by expert (b200q_moe_plan), one buffer of int32. Pair s = t * k + j. A group's pairs keep
 // their order; it is cut into tiles of 128, the row tiles of the activation image.
 //   offsets[E + 1] | order[pairs] (pairs by expert, -1 behind the last) | place[pairs] (tile * 128 + row of pair s, or -1) |
-//   n_tiles, n_units, 2 unused | tiles[max_tiles] {expert, first place in `order`, pairs, 0}, 16-byte aligned |
-//   units[max_units], two neighbouring tiles of an expert or its last one: {expert, first place, pairs, tile} | counts of the ranges
+//   n_tiles, n_units, 2 unused | tiles[max_tiles] {expert, first place in `order`, pairs, first pair}, 16-byte aligned |
+//   units[max_units], two neighbouring tiles of an expert or its last one: {expert, first place, pairs, tile}, {first unit of the expert, its
+//   units, 0, 0} | counts of the ranges
 struct MoePlanLayout {
     size_t order, place, n_tiles, tiles, units, hist, total;
     int64_t max_tiles, max_units;
@@ -47,7 +48,7 @@ inline __host__ MoePlanLayout moe_plan_layout(int64_t pairs, int E) {
     l.n_tiles = (l.place + (size_t)pairs + 3) & ~(size_t)3;
     l.tiles = l.n_tiles + 4;
     l.units = l.tiles + 4 * (size_t)l.max_tiles;
-    l.hist = l.units + 4 * (size_t)l.max_units;
+    l.hist = l.units + 8 * (size_t)l.max_units;
     l.total = l.hist + (size_t)kPlanRanges * (size_t)E;
     return l;
 }

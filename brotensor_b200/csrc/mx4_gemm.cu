@@ -39,7 +39,7 @@ struct MxParams {
     void* Y;
     int* status;
     size_t w_expert_bytes;
-    const int4* tiles;   // grouped: {expert, first place, rows, 0}; nullptr: one matrix, M rows
+    const int4* tiles;   // grouped: {expert, first place, rows, first pair}; nullptr: one matrix, M rows
     const int* n_tiles;
     const int* order;    // grouped: place -> pair, the row of Y
     int pairs_per_row;   // grouped, dense X: pairs that share a row of X (1: X has a row for each pair)
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kMxThreads<XT>, kIsImage<XT> ? 2 : 3) mx4_gemm
     const uint32_t tmem_base = tmem_base_slot;
     if (!p.early || warp != 0) grid_dep_wait();
 
-    int rows = min(p.M - x_tile * kMxTileRows, kMxTileRows), expert = 0, first = x_tile * kMxTileRows;
+    int rows = min(p.M - x_tile * kMxTileRows, kMxTileRows), expert = 0, first = x_tile * kMxTileRows, pair0 = 0;
     if (p.tiles) {
         const int n_tiles = (int)ld_l2_u32(p.n_tiles);
         const uint4 t = ld_l2_u4(p.tiles + x_tile);  // (there is room for every x_tile of the grid)
@@ -118,6 +118,7 @@ __global__ void __launch_bounds__(kMxThreads<XT>, kIsImage<XT> ? 2 : 3) mx4_gemm
         expert = is_tile ? (int)t.x : 0;
         first = (int)t.y;
         rows = is_tile ? (int)t.z : 0;
+        pair0 = (int)t.w;
     }
     const int n_kt = rows > 0 ? share : 0, n_mma = kIsImage<XT> ? (rows + 15) & ~15 : kMxDenseRows;
     int issued = 0;
@@ -199,14 +200,14 @@ __global__ void __launch_bounds__(kMxThreads<XT>, kIsImage<XT> ? 2 : 3) mx4_gemm
         const int w = warp - 2;
         if (w < 4) {
             const int i = w * 32 + lane;
-            if (i < rows) row_of[i] = p.tiles ? (int)ld_l2_u32(p.order + first + i) : first + i;
+            if (i < rows) row_of[i] = !p.tiles ? first + i : i ? (int)ld_l2_u32(p.order + first + i) : pair0;
         }
         if constexpr (!kIsImage<XT>) {
         if (n_kt > 0) {
             // lane r: the row of X of activation row r
             int my_src = lane;
-            if (p.tiles && lane < rows) {
-                my_src = (int)ld_l2_u32(p.order + first + lane);
+            if (p.tiles) {
+                my_src = lane && lane < rows ? (int)ld_l2_u32(p.order + first + lane) : pair0;  // (a tile of one pair, as most are: no load)
                 if (p.pairs_per_row > 1) my_src /= p.pairs_per_row;
             }
             // A warp quantises 256 columns of a row at a time, lane 4 b + s elements 8 s .. 8 s + 7 of block b, with the next row's loads under way.

@@ -31,7 +31,7 @@ struct WideParams {
     void* Y;
     int* status;
     size_t w_expert_bytes;
-    const int4* units;     // grouped: {expert, first place, rows, first tile} of two neighbouring tiles; nullptr: one matrix
+    const int4* units;     // grouped: {expert, first place, rows, first tile}, {first unit, units of the expert, ..} of two neighbouring tiles; nullptr: one matrix
     const int* n_units;
     const int* order;
     int M, N, K, k_tiles;
@@ -125,8 +125,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
     auto item_of = [&](int i, Item& it) {
         int unit;
         if (p.units) {
-            unit = i / p.w_tiles;
-            it.w_tile = i - unit * p.w_tiles;
+            // An expert's items are neighbours, all its units on one tile of weights, then on the next: the weights come from HBM once, at an even rate.
+            const uint4 run = ld_l2_u4(p.units + 2 * (i / p.w_tiles) + 1);
+            const int in = i - (int)run.x * p.w_tiles;
+            it.w_tile = in / (int)run.y;
+            unit = (int)run.x + in - it.w_tile * (int)run.y;
         } else {
             const int per = kGroup * p.w_tiles, g = i / per, in = i - g * per, size = min(kGroup, units - g * kGroup);
             it.w_tile = in / size;
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
         it.first = it.x_tile * kMxTileRows;
         it.rows = p.M - it.first;
         if (p.units) {
-            const uint4 u = ld_l2_u4(p.units + unit);
+            const uint4 u = ld_l2_u4(p.units + 2 * unit);
             it.expert = (int)u.x;
             it.first = (int)u.y + (int)crank * kMxTileRows;
             it.rows = (int)u.z - (int)crank * kMxTileRows;
