@@ -21,6 +21,8 @@ static bool dtype_ok(int dt) { return dt == B200Q_DT_F32 || dt == B200Q_DT_F16 |
 static size_t dtype_size(int dt) { return dt == B200Q_DT_F32 ? 4 : 2; }
 static bool on(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+constexpr int kMostRows = 1 << 30;  // of a dense product: row numbers stay inside 31 bits in whole pairs of tiles
+
 static int check_k(const char* op, int K) {
     if (K <= 0 || K % 32) return fail(B200Q_ERR_BAD_ARG, "%s: K (%d) must be a positive multiple of 32", op, K);
     return B200Q_OK;
@@ -89,6 +91,7 @@ int b200q_mx4_gemm(const void* W, const void* X_image, const void* bias, int bia
     if (!dtype_ok(y_dtype) || !dtype_ok(bias_dtype)) return fail(B200Q_ERR_BAD_ARG, "mx4_gemm: unknown dtype (y %d, bias %d)", y_dtype, bias_dtype);
     if (int rc = check_k("mx4_gemm", K)) return rc;
     if (M < 0 || N < 0) return fail(B200Q_ERR_BAD_ARG, "mx4_gemm: negative shape (M %d, N %d)", M, N);
+    if (M > kMostRows) return fail(B200Q_ERR_UNSUPPORTED, "mx4_gemm: M (%d) is more than %d", M, kMostRows);
     if (M == 0 || N == 0) return B200Q_OK;
     if (int rc = check_product("mx4_gemm", W, X_image, bias, bias_dtype, Y, y_dtype)) return rc;
     int sms, *status;
@@ -108,6 +111,7 @@ int b200q_mx4_linear(const void* W, const void* X, int x_dtype, const void* bias
     if (!dtype_ok(x_dtype) || !dtype_ok(y_dtype)) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: unknown dtype (x %d, y %d)", x_dtype, y_dtype);
     if (int rc = check_k("mx4_linear", K)) return rc;
     if (M < 0 || N < 0) return fail(B200Q_ERR_BAD_ARG, "mx4_linear: negative shape (M %d, N %d)", M, N);
+    if (M > kMostRows) return fail(B200Q_ERR_UNSUPPORTED, "mx4_linear: M (%d) is more than %d", M, kMostRows);
     if (M == 0 || N == 0) return B200Q_OK;
     if (int rc = check_product("mx4_linear", W, X, bias, x_dtype, Y, y_dtype)) return rc;
     if (int rc = check_ws("mx4_linear", ws, ws_bytes, b200q_mx4_linear_workspace_bytes(M, K))) return rc;

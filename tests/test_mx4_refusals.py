@@ -73,7 +73,7 @@ def test_mx4_arguments(L, p):
     g = lambda W=p, X=p, b=None, bt=f32, Y=p, yt=f32, M=1, N=4, K=32: L.b200q_mx4_gemm(W, X, b, bt, Y, yt, M, N, K, None)
     assert g(W=None) == BAD and g(X=p + 8) == BAD and g(Y=p + 2) == BAD and g(yt=3) == BAD and g(bt=7) == BAD
     assert g(b=p + 1, bt=capi.F16) == BAD and g(M=-1) == BAD and g(N=-1) == BAD and g(K=16) == BAD
-    assert g(M=0) == OK and g(N=0) == OK
+    assert g(M=0) == OK and g(N=0) == OK and g(M=2 ** 30 + 1) == UNSUP
     lin = lambda X=p, ws=p, n=1 << 20, M=20, K=32, xt=f32: L.b200q_mx4_linear(p, X, xt, None, p, f32, M, 4, K, ws, n, None)
     assert lin(ws=None) == WS and lin(n=17407) == WS and lin(ws=p + 16) == WS and b"17408 bytes" in L.b200q_last_error()
     assert lin(X=p + 4) == BAD and lin(X=None) == BAD and lin(xt=5) == BAD and lin(K=8) == BAD and lin(M=-3) == BAD and lin(M=0, ws=None) == OK
