@@ -331,6 +331,96 @@ void embedding_impl(const Tensor& table, const std::int32_t* d_idx, int B, Tenso
                                         static_cast<int>(out.dtype), cuda_current_stream(table.device.index)), op);
 }
 
+// ---- MXFP4 and expert layers ----
+constexpr int kMxTileBytes = 17408;  // b200q_mx4_image_bytes(1..128, 32..256)
+
+void mxfp4_pack_impl(const Tensor& W, int experts, Tensor& image) {
+    const char* op = "mxfp4_pack";
+    check_w(W, Dtype::MXFP4, "MXFP4", 32, op);
+    if (experts < 1 || W.rows % experts) op_fail(op, "W.rows must be a multiple of the number of experts");
+    const std::size_t tiles = b200q_mx4_image_bytes(W.rows / experts, W.cols) / kMxTileBytes * static_cast<std::size_t>(experts);
+    if (tiles * kMxTileBytes > 0x7FFFFFFFull) op_fail(op, "the image is larger than a Tensor holds (2^31 elements): pack fewer experts at a time");
+    const int rows = static_cast<int>(tiles);
+    if (image.rows != rows || image.cols != kMxTileBytes || image.dtype != Dtype::INT8 || !image.data) image.resize(rows, kMxTileBytes, Dtype::INT8);
+    check_status(b200q_mx4_pack(W.data, experts, W.rows / experts, W.cols, image.data, cuda_current_stream(W.device.index)), op);
+}
+void check_image(const Tensor& image, int experts, int out, int in, const char* op) {
+    if (out < 0 || experts < 1 || in <= 0 || in % 32) op_fail(op, "in must be a multiple of 32, out and experts must not be negative");
+    if (image.dtype != Dtype::INT8 || image.bytes() < static_cast<std::size_t>(experts) * b200q_mx4_image_bytes(out, in))
+        op_fail(op, "the weights must be an image of these matrices (mxfp4_pack)");
+}
+void check_bias(const Tensor* bias, const Tensor& X, int n, const char* op) {
+    if (!bias) return;
+    if (bias->dtype != X.dtype) op_fail(op, "bias must have X's dtype");
+    if (bias->size() != n) op_fail(op, "bias must have a value for each output");
+}
+// (rows, cols) of FP32 / FP16 / BF16, kept if it is there already
+void size_out(Tensor& y, int rows, int cols, Dtype x_dtype) {
+    if (y.rows != rows || y.cols != cols || !act_dtype(y.dtype) || !y.data) y.resize(rows, cols, x_dtype == Dtype::FP16 ? Dtype::FP16 : Dtype::FP32);
+}
+void mxfp4_linear_impl(const Tensor& image, int out, const Tensor* bias, const Tensor& X, Tensor& Y) {
+    const char* op = "mxfp4_linear_forward";
+    if (!act_dtype(X.dtype)) op_fail(op, "X must be FP16, FP32 or BF16");
+    check_image(image, 1, out, X.cols, op);
+    check_bias(bias, X, out, op);
+    size_out(Y, X.rows, out, X.dtype);
+    if (X.rows == 0 || out == 0) return;
+    const int dev = image.device.index;
+    const std::size_t need = b200q_mx4_linear_workspace_bytes(X.rows, X.cols);
+    const StreamScratch ws(need, cur_stream(dev));
+    check_status(b200q_mx4_linear(image.data, X.data, static_cast<int>(X.dtype), bias ? bias->data : nullptr, Y.data, static_cast<int>(Y.dtype), X.rows, out,
+                                  X.cols, ws.p, need, cuda_current_stream(dev)), op);
+}
+void moe_route_impl(const Tensor& logits, int k, bool normalize, float scale, Tensor& ids, Tensor& weights, Tensor& plan) {
+    const char* op = "moe_route_forward";
+    if (!act_dtype(logits.dtype)) op_fail(op, "logits must be FP16, FP32 or BF16");
+    const int T = logits.rows, E = logits.cols;
+    const std::size_t bytes = b200q_moe_plan_bytes(T, k, E);
+    if (!bytes) op_fail(op, "1 to 1024 experts and 1 to 32 of them for a token are supported");
+    if (ids.rows != T || ids.cols != k || ids.dtype != Dtype::INT32 || !ids.data) ids.resize(T, k, Dtype::INT32);
+    if (weights.rows != T || weights.cols != k || weights.dtype != Dtype::FP32 || !weights.data) weights.resize(T, k, Dtype::FP32);
+    const int n = static_cast<int>(bytes / 4);
+    if (plan.rows != n || plan.cols != 1 || plan.dtype != Dtype::INT32 || !plan.data) plan.resize(n, 1, Dtype::INT32);
+    check_status(b200q_moe_route(logits.data, static_cast<int>(logits.dtype), T, E, k, normalize ? 1 : 0, scale, static_cast<int32_t*>(ids.data),
+                                 static_cast<float*>(weights.data), plan.data, cuda_current_stream(logits.device.index)), op);
+}
+void moe_product(const char* op, const Tensor& image, const Tensor* up, int experts, int out, const Tensor* bias, const Tensor& X, const Tensor& plan, int tokens,
+                 int k, Tensor& Y) {
+    if (!act_dtype(X.dtype)) op_fail(op, "X must be FP16, FP32 or BF16");
+    check_image(image, experts, out, X.cols, op);
+    if (up) check_image(*up, experts, out, X.cols, op);
+    const std::size_t bytes = b200q_moe_plan_bytes(tokens, k, experts);
+    if (!bytes || plan.dtype != Dtype::INT32 || plan.bytes() < bytes) op_fail(op, "the plan must be of these tokens, k and experts (moe_route_forward)");
+    if (X.rows != tokens && X.rows != tokens * k) op_fail(op, "X must have a row for each token or for each token and choice");
+    check_bias(bias, X, experts * out, op);
+    size_out(Y, tokens * k, out, X.dtype);
+    if (tokens == 0 || out == 0) return;
+    const int dev = image.device.index, per_pair = X.rows != tokens;
+    const std::size_t need = b200q_moe_mx4_workspace_bytes(tokens, k, experts, X.cols);
+    const StreamScratch ws(need, cur_stream(dev));
+    void* st = cuda_current_stream(dev);
+    const int xt = static_cast<int>(X.dtype), yt = static_cast<int>(Y.dtype);
+    check_status(up ? b200q_moe_mx4_swiglu(image.data, up->data, X.data, xt, per_pair, plan.data, Y.data, yt, tokens, k, experts, out, X.cols, ws.p, need, st)
+                    : b200q_moe_mx4_linear(image.data, X.data, xt, per_pair, plan.data, bias ? bias->data : nullptr, Y.data, yt, tokens, k, experts, out, X.cols,
+                                           ws.p, need, st), op);
+}
+void moe_linear_impl(const Tensor& image, int experts, int out, const Tensor* bias, const Tensor& X, const Tensor& plan, int tokens, int k, Tensor& Y) {
+    moe_product("moe_linear_forward", image, nullptr, experts, out, bias, X, plan, tokens, k, Y);
+}
+void moe_swiglu_impl(const Tensor& gate, const Tensor& up, int experts, int out, const Tensor& X, const Tensor& plan, int tokens, int k, Tensor& Y) {
+    moe_product("moe_swiglu_forward", gate, &up, experts, out, nullptr, X, plan, tokens, k, Y);
+}
+void moe_combine_impl(const Tensor& Y, const Tensor& ids, const Tensor& weights, int experts, Tensor& out) {
+    const char* op = "moe_combine_forward";
+    if (!act_dtype(Y.dtype)) op_fail(op, "Y must be FP16, FP32 or BF16");
+    const int T = ids.rows, k = ids.cols;
+    if (ids.dtype != Dtype::INT32 || weights.dtype != Dtype::FP32 || weights.rows != T || weights.cols != k) op_fail(op, "ids must be INT32 and weights FP32, both (T, k)");
+    if (k < 1 || Y.rows != T * k) op_fail(op, "Y must have a row for each token and choice");
+    if (out.rows != T || out.cols != Y.cols || out.dtype != Y.dtype || !out.data) out.resize(T, Y.cols, Y.dtype);
+    check_status(b200q_moe_combine(Y.data, static_cast<int>(Y.dtype), static_cast<const int32_t*>(ids.data), static_cast<const float*>(weights.data), T, k, experts,
+                                   Y.cols, out.data, cuda_current_stream(Y.device.index)), op);
+}
+
 }  // namespace
 
 // The registration point: what brotensor does in fill_cuda_vtable_specialised
@@ -352,6 +442,12 @@ void fill_cuda_tables(OpsVTable& ops, AllocVTable& alloc) {
     ops.linear_forward_q5k_fp16 = gemv_q5k;
     ops.linear_forward_batched_q5k_fp16 = batched_q5k;
     ops.embedding_lookup_forward = embedding_impl;
+    ops.mxfp4_pack = mxfp4_pack_impl;
+    ops.mxfp4_linear_forward = mxfp4_linear_impl;
+    ops.moe_route_forward = moe_route_impl;
+    ops.moe_linear_forward = moe_linear_impl;
+    ops.moe_swiglu_forward = moe_swiglu_impl;
+    ops.moe_combine_forward = moe_combine_impl;
     ops.dequant_q6k_to_fp16 = dequant_q6k;
     ops.linear_forward_q6k_fp16 = gemv_q6k;
     ops.linear_forward_batched_q6k_fp16 = batched_q6k;

@@ -54,6 +54,7 @@ TypeRow type_row(std::uint32_t t) {
         case 14: return {Dtype::Q6_K, true, 256, 210};
         case 15: return {Dtype::Q8_K, true, 256, 292};
         case 30: return {Dtype::BF16, true, 1, 2};
+        case 39: return {Dtype::MXFP4, true, 32, 17};
         default: return {Dtype::FP32, false, 0, 0};
     }
 }

@@ -4,6 +4,7 @@
 #include <string>
 
 #include "brotensor_b200/detail/dispatch.h"
+#include "brotensor_b200/ops/experts.h"
 #include "brotensor_b200/ops/quant.h"
 
 namespace brotensor_b200 {
@@ -87,6 +88,45 @@ void linear_forward_swiglu_fp16(const Tensor& W_gate, const Tensor& W_up, const 
     if (!v.linear_forward_swiglu_fp16) detail::throw_not_implemented("linear_forward_swiglu_fp16", W_gate.device);
     detail::adopt_output(y, W_gate.device);
     v.linear_forward_swiglu_fp16(W_gate, W_up, x, y);
+}
+
+void mxfp4_pack(const Tensor& W, int experts, Tensor& image) {
+    const detail::OpsVTable& v = detail::dispatch_with_opts(W, {&image});
+    if (!v.mxfp4_pack) detail::throw_not_implemented("mxfp4_pack", W.device);
+    detail::adopt_output(image, W.device);
+    v.mxfp4_pack(W, experts, image);
+}
+void mxfp4_linear_forward(const Tensor& image, int out, const Tensor* bias, const Tensor& X, Tensor& Y) {
+    const detail::OpsVTable& v = detail::dispatch_with_opts(image, {bias, &X, &Y});
+    if (!v.mxfp4_linear_forward) detail::throw_not_implemented("mxfp4_linear_forward", image.device);
+    detail::adopt_output(Y, image.device);
+    v.mxfp4_linear_forward(image, out, bias, X, Y);
+}
+void moe_route_forward(const Tensor& logits, int k, bool normalize, float scale, Tensor& ids, Tensor& weights, Tensor& plan) {
+    const detail::OpsVTable& v = detail::dispatch_with_opts(logits, {&ids, &weights, &plan});
+    if (!v.moe_route_forward) detail::throw_not_implemented("moe_route_forward", logits.device);
+    detail::adopt_output(ids, logits.device);
+    detail::adopt_output(weights, logits.device);
+    detail::adopt_output(plan, logits.device);
+    v.moe_route_forward(logits, k, normalize, scale, ids, weights, plan);
+}
+void moe_linear_forward(const Tensor& image, int experts, int out, const Tensor* bias, const Tensor& X, const Tensor& plan, int tokens, int k, Tensor& Y) {
+    const detail::OpsVTable& v = detail::dispatch_with_opts(image, {bias, &X, &plan, &Y});
+    if (!v.moe_linear_forward) detail::throw_not_implemented("moe_linear_forward", image.device);
+    detail::adopt_output(Y, image.device);
+    v.moe_linear_forward(image, experts, out, bias, X, plan, tokens, k, Y);
+}
+void moe_swiglu_forward(const Tensor& gate, const Tensor& up, int experts, int out, const Tensor& X, const Tensor& plan, int tokens, int k, Tensor& Y) {
+    const detail::OpsVTable& v = detail::dispatch_with_opts(gate, {&up, &X, &plan, &Y});
+    if (!v.moe_swiglu_forward) detail::throw_not_implemented("moe_swiglu_forward", gate.device);
+    detail::adopt_output(Y, gate.device);
+    v.moe_swiglu_forward(gate, up, experts, out, X, plan, tokens, k, Y);
+}
+void moe_combine_forward(const Tensor& Y, const Tensor& ids, const Tensor& weights, int experts, Tensor& out) {
+    const detail::OpsVTable& v = detail::dispatch_with_opts(Y, {&ids, &weights, &out});
+    if (!v.moe_combine_forward) detail::throw_not_implemented("moe_combine_forward", Y.device);
+    detail::adopt_output(out, Y.device);
+    v.moe_combine_forward(Y, ids, weights, experts, out);
 }
 
 }  // namespace brotensor_b200

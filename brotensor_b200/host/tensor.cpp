@@ -38,6 +38,7 @@ DtInfo dt_info(Dtype d) {
         case Dtype::Q5_K: return {0, 256, 176};
         case Dtype::Q6_K: return {0, 256, 210};
         case Dtype::Q8_K: return {0, 256, 292};
+        case Dtype::MXFP4: return {0, 32, 17};
     }
     throw std::runtime_error("brotensor: unknown dtype");
 }

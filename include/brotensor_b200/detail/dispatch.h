@@ -45,6 +45,15 @@ struct OpsVTable {
     // Extension: the grouped op on rms_norm(x) * gamma, the normalisation folded into the launch.
     void (*linear_forward_group_rmsnorm_fp16)(const Tensor* const* W, int n, const Tensor& x, const Tensor& gamma, float eps,
                                               Tensor* const* y) = nullptr;
+    // Extension: MXFP4 weights and expert layers on them (ops/experts.h).
+    void (*mxfp4_pack)(const Tensor& W, int experts, Tensor& image) = nullptr;
+    void (*mxfp4_linear_forward)(const Tensor& image, int out, const Tensor* bias, const Tensor& X, Tensor& Y) = nullptr;
+    void (*moe_route_forward)(const Tensor& logits, int k, bool normalize, float scale, Tensor& ids, Tensor& weights, Tensor& plan) = nullptr;
+    void (*moe_linear_forward)(const Tensor& image, int experts, int out, const Tensor* bias, const Tensor& X, const Tensor& plan, int tokens, int k,
+                               Tensor& Y) = nullptr;
+    void (*moe_swiglu_forward)(const Tensor& gate, const Tensor& up, int experts, int out, const Tensor& X, const Tensor& plan, int tokens, int k,
+                               Tensor& Y) = nullptr;
+    void (*moe_combine_forward)(const Tensor& Y, const Tensor& ids, const Tensor& weights, int experts, Tensor& out) = nullptr;
 };
 
 struct AllocVTable {

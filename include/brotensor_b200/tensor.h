@@ -20,6 +20,7 @@ enum class Dtype : int {
     FP32 = 0, FP16 = 1, INT8 = 2, INT32 = 3, BF16 = 4, F64 = 5,
     Q4_0 = 10, Q4_1 = 11, Q5_0 = 12, Q5_1 = 13, Q8_0 = 14, Q8_1 = 15,
     Q2_K = 20, Q3_K = 21, Q4_K = 22, Q5_K = 23, Q6_K = 24, Q8_K = 25,
+    MXFP4 = 139,  // ggml block_mxfp4 (type 39): not in brotensor; 32 elements / 17 B, taken by the ops of ops/experts.h
 };
 
 int dtype_size_bytes(Dtype);   // bytes per scalar; 0 for block-quant carriers
