@@ -23,8 +23,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 def _launch(t: torch.Tensor, f, *args) -> int:
     """f(*args, stream) with t's device current; the device is switched only when it is another one (entering and leaving
     torch.cuda.device and wrapping the stream in an object were a third of a small call's time on the host)."""
-    i = t.device.index
-    if i is not None and i == _current_device():
+    i = t.get_device()  # -1: not on a CUDA device
+    if i >= 0 and i == _current_device():
         return f(*args, _raw_stream(i))
     with torch.cuda.device(t.device):  # refuses a tensor that is not on a CUDA device
         return f(*args, _raw_stream(i))
@@ -179,8 +179,8 @@ def linear(fmt, W, X, N, bias=None, out=None, out_dtype=None, ws=None):
 
 # ---- MXFP4 matrices and sparse expert layers on them -------------------------------------------------------
 
-# (The wrappers below are written for short calls: a decode step makes a dozen of them per layer, and at a few microseconds each every torch
-# call on the way counts.)
+# (The wrappers below are written for short calls: a decode step makes a dozen of them per layer, and at a few microseconds each every call on the
+# way counts. They look at everything in one condition and go to the checks that say what is wrong only where it fails.)
 
 def mx4_image_bytes(rows: int, K: int) -> int:
     """Bytes of the image of a rows x K matrix in MXFP4 (K a multiple of 32)."""
@@ -197,6 +197,11 @@ def _check_image(W: torch.Tensor, rows: int, K: int, count: int = 1) -> int:
     if W.numel() < count * mx4_image_bytes(rows, K):
         raise ValueError(f"the image holds {W.numel()} bytes, {count} x ({rows}, {K}) needs {count * mx4_image_bytes(rows, K)}")
     return device
+
+
+def _is_image(W: torch.Tensor, rows: int, K: int, count: int, device: int) -> bool:
+    return (W.dtype is torch.uint8 and W.get_device() == device >= 0 and K > 0 and not K & 31 and rows >= 0 and W.is_contiguous()
+            and W.numel() >= count * ((rows + 127) >> 7) * ((K + 255) >> 8) * 17408)
 
 
 def _check_dense(t: torch.Tensor, what: str, device: int) -> int:
@@ -256,8 +261,9 @@ def mx4_quantize(x: torch.Tensor, out=None) -> torch.Tensor:
     """(rows, K) float32 / float16 / bfloat16 -> image."""
     if x.dim() != 2:
         raise ValueError("x must be (rows, K)")
-    device = x.get_device()
-    code = _check_dense(x, "x", device)
+    device, code = x.get_device(), _DT.get(x.dtype)
+    if code is None or device < 0 or not x.is_contiguous():
+        _check_dense(x, "x", device)
     rows, K = x.shape
     size = mx4_image_bytes(rows, K)
     if out is None:
@@ -270,7 +276,8 @@ def mx4_quantize(x: torch.Tensor, out=None) -> torch.Tensor:
 
 def mx4_dequantize(image: torch.Tensor, rows: int, K: int, out_dtype=torch.float32) -> torch.Tensor:
     """The values of an image, (rows, K)."""
-    _check_image(image, rows, K)
+    if not _is_image(image, rows, K, 1, image.get_device()):
+        _check_image(image, rows, K)
     code = _DT.get(out_dtype)
     if code is None:
         raise ValueError("out_dtype must be float32, float16 or bfloat16")
@@ -305,8 +312,10 @@ def mx4_linear(W: torch.Tensor, X: torch.Tensor, N: int, bias=None, out=None, ou
     if X.dim() != 2:
         raise ValueError("X must be (M, K)")
     M, K = X.shape
-    device = _check_image(W, N, K)
-    code = _check_dense(X, "X", device)
+    device, code = X.get_device(), _DT.get(X.dtype)
+    if code is None or not X.is_contiguous() or not _is_image(W, N, K, 1, device):
+        _check_dense(X, "X", _check_image(W, N, K))
+        raise ValueError("W and X are on different devices")
     bias_ptr = None
     if bias is not None:
         if _check_dense(bias, "bias", device) != code or bias.numel() != N:
@@ -317,7 +326,8 @@ def mx4_linear(W: torch.Tensor, X: torch.Tensor, N: int, bias=None, out=None, ou
     else:
         _check_out(out, (M, N), out_dtype, device)
     L = capi.lib()
-    ws_ptr, ws_bytes, ws = _scratch(ws, L.b200q_mx4_linear_workspace_bytes(M, K), X)
+    need = L.b200q_mx4_linear_workspace_bytes(M, K)
+    ws_ptr, ws_bytes, ws = _scratch(ws, need, X) if need or ws is not None else (None, 0, None)
     capi.check(_launch(X, L.b200q_mx4_linear, W.data_ptr(), X.data_ptr(), code, bias_ptr, out.data_ptr(), _DT[out.dtype], M, N, K, ws_ptr, ws_bytes))
     return out
 
@@ -337,11 +347,11 @@ class MoePlan:
 
     @property
     def offsets(self) -> torch.Tensor:
-        return self.data[:self.experts + 1]
+        return self.data.as_strided((self.experts + 1,), (1,), 0)
 
     @property
     def order(self) -> torch.Tensor:
-        return self.data[self.experts + 1:self.experts + 1 + self.tokens * self.k]
+        return self.data.as_strided((self.tokens * self.k,), (1,), self.experts + 1)
 
 
 def moe_plan(ids: torch.Tensor, experts: int) -> MoePlan:
@@ -359,7 +369,9 @@ def moe_route(logits: torch.Tensor, k: int, normalize: bool = True, scale: float
     weights over the chosen (normalize) or over all experts, times scale; the grouping by expert."""
     if logits.dim() != 2:
         raise ValueError("logits must be a (tokens, E) CUDA tensor")
-    code = _check_dense(logits, "logits", logits.get_device())
+    code = _DT.get(logits.dtype)
+    if code is None or logits.get_device() < 0 or not logits.is_contiguous():
+        _check_dense(logits, "logits", logits.get_device())
     T, E = logits.shape
     device = logits.device
     plan = MoePlan(T, k, E, device)
@@ -376,16 +388,19 @@ def _moe_common(Ws, X, plan, N, out, out_dtype, ws):
     shape = X.shape
     if (len(shape) != 2 and (len(shape) != 3 or shape[1] != k)) or shape[0] != T:
         raise ValueError(f"X must be ({T}, K) or ({T}, {k}, K), as the plan")
-    device, K = plan.data.get_device(), shape[-1]
-    code = _check_dense(X, "X", device)
+    device, K, code = plan.data.get_device(), shape[-1], _DT.get(X.dtype)
+    if code is None or X.get_device() != device or not X.is_contiguous():
+        _check_dense(X, "X", device)
     for W in Ws:
-        if _check_image(W, N, K, E) != device:
+        if not _is_image(W, N, K, E, device):
+            _check_image(W, N, K, E)
             raise ValueError("the weights are on another device than X")
     if out is None:
         out = torch.empty(T, k, N, dtype=out_dtype or _default_out(X), device=X.device)
     else:
         _check_out(out, (T, k, N), out_dtype, device)
-    return code, len(shape) - 2, out, K, _scratch(ws, capi.lib().b200q_moe_mx4_workspace_bytes(T, k, E, K), X)
+    need = capi.lib().b200q_moe_mx4_workspace_bytes(T, k, E, K)
+    return code, len(shape) - 2, out, K, _scratch(ws, need, X) if need or ws is not None else (None, 0, None)
 
 
 def moe_mx4_linear(W, X, plan: MoePlan, N: int, bias=None, out=None, out_dtype=None, ws=None) -> torch.Tensor:
@@ -415,11 +430,12 @@ def moe_combine(y: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, exper
     if y.dim() != 3:
         raise ValueError("y must be a (tokens, k, N) CUDA tensor")
     T, k, N = y.shape
-    device = y.get_device()
-    code = _check_dense(y, "y", device)
-    _check_int32(ids, "ids", (T, k), device)
-    if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.shape != (T, k) or weights.get_device() != device:
-        raise ValueError(f"weights must be a contiguous float32 tensor of shape {(T, k)} on {y.device}")
+    device, code, pairs = y.get_device(), _DT.get(y.dtype), (T, k)
+    if (code is None or device < 0 or ids.dtype is not torch.int32 or weights.dtype is not torch.float32 or ids.shape != pairs or weights.shape != pairs
+            or ids.get_device() != device or weights.get_device() != device or not (y.is_contiguous() and ids.is_contiguous() and weights.is_contiguous())):
+        _check_dense(y, "y", device)
+        _check_int32(ids, "ids", pairs, device)
+        raise ValueError(f"weights must be a contiguous float32 tensor of shape {pairs} on {y.device}")
     if out is None:
         out = torch.empty(T, N, dtype=y.dtype, device=y.device)
     else:
