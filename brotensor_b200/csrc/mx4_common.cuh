@@ -12,6 +12,8 @@
 // another row's results).
 #pragma once
 
+#include <type_traits>
+
 #include "gemm_common.cuh"
 
 namespace b200q {
@@ -71,29 +73,44 @@ __device__ __forceinline__ uint32_t mx_scale_offset(int r, int half) { return (u
 // Quantisation (OCP Microscaling Formats specification 1.0, 6.3): a block's exponent is floor(log2(largest magnitude)) - 2, which puts
 // the largest magnitude into [4, 8); elements are divided by that power of two - exact in FP32 - and rounded to the nearest E2M1
 // value, ties to the even one, magnitudes beyond 6 to 6. A block with an infinity or a NaN becomes NaN as a whole (e = 255), one of zeros e = 0.
-// Eight neighbouring elements in FP32.
+// Eight neighbouring elements of a row as they lie in memory: four or eight registers.
 template <typename T>
-__device__ __forceinline__ void mx_load8(const T* p, float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = ld_dep_f4(p), b = ld_dep_f4(p + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        union {
-            uint4 q;
-            T e[8];
-        } u;
-        u.q = ld_dep_u4(p);
+struct MxEight {
+    uint4 q[sizeof(T) / 2];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(u.e[i]);
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = make_uint4(0, 0, 0, 0);
     }
-}
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = ld_dep_u4(p + i * 16 / sizeof(T));
+    }
+    // Largest magnitude as the bits of an FP32: without their signs, bits compare like the magnitudes, infinities and NaNs above all. 16-bit types go two at a time.
+    __device__ __forceinline__ uint32_t top() const {
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t m = 0x7FFFFFFFu;
+            return max(max(max(q[0].x & m, q[0].y & m), max(q[0].z & m, q[0].w & m)), max(max(q[1].x & m, q[1].y & m), max(q[1].z & m, q[1].w & m)));
+        } else {
+            const uint32_t m = 0x7FFF7FFFu, two = __vmaxu2(__vmaxu2(q[0].x & m, q[0].y & m), __vmaxu2(q[0].z & m, q[0].w & m));
+            const uint32_t one = max(two & 0xFFFFu, two >> 16);
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) return one << 16;
+            else return __float_as_uint(h2f(one));
+        }
+    }
+    __device__ __forceinline__ float get(int j) const {  // j is known when this is compiled
+        const uint4& v = q[sizeof(T) == 4 ? j >> 2 : 0];
+        const int i = sizeof(T) == 4 ? j & 3 : j >> 1;
+        const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
+        else return h2f(j & 1 ? w >> 16 : w & 0xFFFFu);
+    }
+};
 
 // A quad of lanes holds a block, eight elements each: returns the lane's eight nibbles and the block's scale byte.
-__device__ __forceinline__ uint32_t mx_quantise8(const float (&v)[8], uint32_t& scale) {
-    uint32_t top = 0;  // magnitudes as bits compare like magnitudes, infinities and NaNs above all
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+template <typename T>
+__device__ __forceinline__ uint32_t mx_quantise8(const MxEight<T>& v, uint32_t& scale) {
+    uint32_t top = v.top();
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int be = (int)(top >> 23);  // 0: a zero or a subnormal, below 2^-126 - the smallest scale serves
@@ -113,7 +130,7 @@ __device__ __forceinline__ uint32_t mx_quantise8(const float (&v)[8], uint32_t& 
         "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
         "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
         : "=r"(out)
-        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
+        : "f"(v.get(0) * inv), "f"(v.get(1) * inv), "f"(v.get(2) * inv), "f"(v.get(3) * inv), "f"(v.get(4) * inv), "f"(v.get(5) * inv), "f"(v.get(6) * inv), "f"(v.get(7) * inv));
     return out;
 }
 

@@ -264,14 +264,14 @@ __global__ void __launch_bounds__(kMxThreads<XT>, kIsImage<XT> ? 2 : 3) mx4_gemm
                         const int k = (kt0 + kt) * kMxTileK + 8 * lane;
                         const XT* x = static_cast<const XT*>(p.X) + k;
                         const uint32_t at = x_base + (uint32_t)kt * x_step, to = at + kMxSfBytes + 4 * s, sc_to = at + (uint32_t)((lane >> 4) * 512);
-                        float v[8], next[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] = next[j] = 0.f;
+                        MxEight<XT> v, next;
+                        v.clear();
+                        next.clear();
                         int64_t src = __shfl_sync(0xffffffffu, my_src, r0 & 31);
-                        if (r0 < it.rows && k < p.K) mx_load8(x + src * p.K, v);
+                        if (r0 < it.rows && k < p.K) v.load(x + src * p.K);
                         for (int r = r0; r < it.rows; r += abreast) {
                             src = __shfl_sync(0xffffffffu, my_src, (r + abreast) & 31);
-                            if (r + abreast < it.rows && k < p.K) mx_load8(x + src * p.K, next);
+                            if (r + abreast < it.rows && k < p.K) next.load(x + src * p.K);
                             uint32_t sc;
                             const uint32_t q = mx_quantise8(v, sc);
                             uint32_t word = sc << (8 * (b & 3));
@@ -279,8 +279,7 @@ __global__ void __launch_bounds__(kMxThreads<XT>, kIsImage<XT> ? 2 : 3) mx4_gemm
                             word |= __shfl_xor_sync(0xffffffffu, word, 8);
                             sts32(to + (uint32_t)(r >> 3) * 1024u + (uint32_t)(r & 7) * 128u + ((uint32_t)(b ^ (r & 7)) << 4), q);
                             if ((lane & 15) == 0) sts32(sc_to + (uint32_t)r * 16u, word);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] = next[j];
+                            v = next;
                         }
                     }
                 }

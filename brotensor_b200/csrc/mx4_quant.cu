@@ -30,12 +30,11 @@ __global__ void __launch_bounds__(kQuantThreads) mx4_quantise_kernel(const T* x,
     const Patch at(wide, kBatch);
     if (at.row >= rows || at.kt >= k_tiles) return;
     const T* src = x + at.row * K + (int64_t)at.kt * kMxTileK + 8 * lane;
-    float v[kBatch][8];
+    MxEight<T> v[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
-        if ((at.kt + u) * kMxTileK + 8 * lane < K) mx_load8(src + u * kMxTileK, v[u]);
+        v[u].clear();
+        if ((at.kt + u) * kMxTileK + 8 * lane < K) v[u].load(src + u * kMxTileK);
     }
     uint32_t q[kBatch], word[kBatch];
 #pragma unroll
