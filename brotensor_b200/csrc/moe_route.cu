@@ -443,7 +443,7 @@ static cudaError_t combine_typed(const void* y, const int* ids, const float* wei
     const int items = wide ? N / V : N;
     // few results: small blocks, so that they spread over the SMs
     const int threads = (int64_t)items * tokens >= (int64_t)sms * kCombineThreads ? kCombineThreads : 64;
-    const dim3 grid((unsigned)((items + threads - 1) / threads), (unsigned)(tokens < 65535 ? tokens : 65535)), block(threads);
+    const dim3 grid(((unsigned)items + threads - 1) / threads, (unsigned)(tokens < 65535 ? tokens : 65535)), block(threads);
     if (wide) return launch_dep(dep, moe_combine_kernel<T, V>, grid, block, 0, st, static_cast<const T*>(y), ids, weights, tokens, k, N, E, static_cast<T*>(out));
     return launch_dep(dep, moe_combine_kernel<T, 1>, grid, block, 0, st, static_cast<const T*>(y), ids, weights, tokens, k, N, E, static_cast<T*>(out));
 }

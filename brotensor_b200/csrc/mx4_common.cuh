@@ -23,7 +23,7 @@ constexpr int kMxQBytes = 16384, kMxSfBytes = 1024, kMxTileBytes = kMxQBytes + k
 constexpr int kMxBlockBytes = 17;  // ggml block_mxfp4: u8 e, u8 qs[16] (low nibbles elements 0..15, high nibbles 16..31)
 constexpr int kMaxExperts = 1024, kMaxExpertsPerToken = 32;
 
-inline __host__ __device__ int mx_k_tiles(int K) { return (K + kMxTileK - 1) / kMxTileK; }
+inline __host__ __device__ int mx_k_tiles(int K) { return K / kMxTileK + (K % kMxTileK != 0); }
 inline __host__ __device__ int64_t mx_row_tiles(int64_t rows) { return (rows + kMxTileRows - 1) / kMxTileRows; }
 inline __host__ __device__ size_t mx_image_bytes(int64_t rows, int K) { return (size_t)mx_row_tiles(rows) * mx_k_tiles(K) * kMxTileBytes; }
 

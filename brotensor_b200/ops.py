@@ -184,8 +184,8 @@ def linear(fmt, W, X, N, bias=None, out=None, out_dtype=None, ws=None):
 
 def mx4_image_bytes(rows: int, K: int) -> int:
     """Bytes of the image of a rows x K matrix in MXFP4 (K a multiple of 32)."""
-    if rows < 0 or K <= 0 or K % 32:
-        raise ValueError(f"K ({K}) must be a positive multiple of 32")
+    if rows < 0 or K <= 0 or K % 32 or K >> 31:
+        raise ValueError(f"K ({K}) must be a positive multiple of 32 below 2^31")
     return ((rows + 127) >> 7) * ((K + 255) >> 8) * 17408
 
 
@@ -200,7 +200,7 @@ def _check_image(W: torch.Tensor, rows: int, K: int, count: int = 1) -> int:
 
 
 def _is_image(W: torch.Tensor, rows: int, K: int, count: int, device: int) -> bool:
-    return (W.dtype is torch.uint8 and W.get_device() == device >= 0 and K > 0 and not K & 31 and rows >= 0 and W.is_contiguous()
+    return (W.dtype is torch.uint8 and W.get_device() == device >= 0 and 0 < K < 2 ** 31 and not K & 31 and rows >= 0 and W.is_contiguous()
             and W.numel() >= count * ((rows + 127) >> 7) * ((K + 255) >> 8) * 17408)
 
 
@@ -339,7 +339,7 @@ class MoePlan:
     __slots__ = ("tokens", "k", "experts", "data")
 
     def __init__(self, tokens: int, k: int, experts: int, device):
-        size = capi.lib().b200q_moe_plan_bytes(tokens, k, experts)
+        size = capi.lib().b200q_moe_plan_bytes(tokens, k, experts) if 0 < k <= 32 and 0 < experts <= 1024 else 0  # (a C int holds no more than 31 bits)
         if not size:
             raise ValueError(f"{tokens} tokens, {k} of {experts} experts each: outside the supported sizes (1..1024 experts, 1..32 each)")
         self.tokens, self.k, self.experts = tokens, k, experts
@@ -430,6 +430,8 @@ def moe_combine(y: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, exper
     if y.dim() != 3:
         raise ValueError("y must be a (tokens, k, N) CUDA tensor")
     T, k, N = y.shape
+    if k >> 31 or N >> 31 or experts >= 1 << 31:
+        raise ValueError(f"k ({k}), N ({N}) and experts ({experts}) must be below 2^31")
     device, code, pairs = y.get_device(), _DT.get(y.dtype), (T, k)
     if (code is None or device < 0 or ids.dtype is not torch.int32 or weights.dtype is not torch.float32 or ids.shape != pairs or weights.shape != pairs
             or ids.get_device() != device or weights.get_device() != device or not (y.is_contiguous() and ids.is_contiguous() and weights.is_contiguous())):

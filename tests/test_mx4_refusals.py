@@ -129,3 +129,19 @@ def test_the_reference_quantises_as_the_format_says():
     want[0, :14] = torch.tensor([6.0, 0.0, 0.5, 1.0, 1.0, 1.5, 2.0, 2.0, 3.0, 4.0, 4.0, 6.0, -4.0, -0.5])
     assert torch.equal(ref.quantise(v), want)
     assert torch.equal(ref.quantise(v * 2 ** -100), want * 2 ** -100)
+
+
+def test_sizes_at_the_end_of_an_int(L):
+    assert L.b200q_mx4_image_bytes(1, 2 ** 31 - 32) == 2 ** 23 * 17408 == ops.mx4_image_bytes(1, 2 ** 31 - 32)
+
+
+def test_python_front_end_refuses_what_a_c_int_does_not_hold():
+    """ctypes would pass the low 32 bits on, and a call with other sizes would be made."""
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.mx4_image_bytes(1, 2 ** 32 + 32)
+    for k, experts in ((2, 2 ** 32 + 8), (2 ** 32 + 2, 8)):
+        with pytest.raises(ValueError, match="supported sizes"):
+            ops.MoePlan(1, k, experts, "cpu")
+    for k, n, experts in ((1, 2 ** 32 + 8, 4), (2 ** 32 + 1, 8, 4), (1, 8, 2 ** 32 + 4)):
+        with pytest.raises(ValueError, match="below 2"):
+            ops.moe_combine(torch.empty(1, k, n, device="meta"), torch.empty(1, k, dtype=torch.int32, device="meta"), torch.empty(1, k, device="meta"), experts)
