@@ -377,6 +377,7 @@ void moe_route_impl(const Tensor& logits, int k, bool normalize, float scale, Te
     const int T = logits.rows, E = logits.cols;
     const std::size_t bytes = b200q_moe_plan_bytes(T, k, E);
     if (!bytes) op_fail(op, "1 to 1024 experts and 1 to 32 of them for a token are supported");
+    if (bytes / 4 > 0x7FFFFFFFu) op_fail(op, "the plan is larger than a Tensor holds (2^31 elements): route fewer tokens at a time");
     if (ids.rows != T || ids.cols != k || ids.dtype != Dtype::INT32 || !ids.data) ids.resize(T, k, Dtype::INT32);
     if (weights.rows != T || weights.cols != k || weights.dtype != Dtype::FP32 || !weights.data) weights.resize(T, k, Dtype::FP32);
     const int n = static_cast<int>(bytes / 4);
@@ -415,7 +416,7 @@ void moe_combine_impl(const Tensor& Y, const Tensor& ids, const Tensor& weights,
     if (!act_dtype(Y.dtype)) op_fail(op, "Y must be FP16, FP32 or BF16");
     const int T = ids.rows, k = ids.cols;
     if (ids.dtype != Dtype::INT32 || weights.dtype != Dtype::FP32 || weights.rows != T || weights.cols != k) op_fail(op, "ids must be INT32 and weights FP32, both (T, k)");
-    if (k < 1 || Y.rows != T * k) op_fail(op, "Y must have a row for each token and choice");
+    if (k < 1 || Y.rows != static_cast<int64_t>(T) * k) op_fail(op, "Y must have a row for each token and choice");
     if (out.rows != T || out.cols != Y.cols || out.dtype != Y.dtype || !out.data) out.resize(T, Y.cols, Y.dtype);
     check_status(b200q_moe_combine(Y.data, static_cast<int>(Y.dtype), static_cast<const int32_t*>(ids.data), static_cast<const float*>(weights.data), T, k, experts,
                                    Y.cols, out.data, cuda_current_stream(Y.device.index)), op);

@@ -214,6 +214,20 @@ static void test_gpu_layer(int T) {
     CHECK(throws_with([&] { bt::moe_route_forward(L, E + 1, true, 1.f, ids, weights, plan); }, "more than E"));
 }
 
+// Sizes whose products leave an int: refused by their numbers alone (views that claim more rows than there is memory behind them).
+static void test_gpu_sizes() {
+    std::printf("test_gpu_sizes\n");
+    const Tensor some = Tensor::zeros_on(Device::cuda(0), 256, 1);
+    const auto claim = [&](int rows, int cols, Dtype dt) { return Tensor::view(Device::cuda(0), some.data, rows, cols, dt); };
+    Tensor ids, weights, plan, out;
+    for (int T : {40000000, 67000000})  // the plan's size in 32-bit words is beyond 2^31 and beyond 2^32
+        CHECK(throws_with([&] { bt::moe_route_forward(claim(T, 32, Dtype::FP16), 32, true, 1.f, ids, weights, plan); }, "larger than a Tensor holds"));
+    CHECK(!ids.data && !plan.data);
+    // 65536 x 65537 pairs are 2^32 + 65536
+    CHECK(throws_with([&] { bt::moe_combine_forward(claim(65536, 1, Dtype::FP32), claim(65536, 65537, Dtype::INT32), claim(65536, 65537, Dtype::FP32), 4, out); },
+                      "a row for each token"));
+}
+
 int main(int argc, char** argv) {
     const std::string mode = argc > 1 ? argv[1] : "cpu";
     bt::init();
@@ -225,6 +239,7 @@ int main(int argc, char** argv) {
     } else {
         test_gpu_linear();
         for (int T : {1, 7, 150}) test_gpu_layer(T);
+        test_gpu_sizes();
         int st = 0;
         CHECK(b200q_device_status(&st) == B200Q_OK && st == 0);
     }
