@@ -170,8 +170,9 @@ static int dequantise_typed(const void* image, int64_t rows, int K, void* out, c
     return B200Q_OK;
 }
 
-// Several column tiles a warp once every SM has 32 warps' worth of single ones: four of 16-bit elements, two of FP32, measured on 14336 x 4096 BF16
-// and 2000 x 4096 FP32 (two, four, eight: 31.9, 27.3, 28.8 us and 6.5, 6.8, 7.6; back 26.5, 24.9, 26.8 and, with 16-byte stores, 10.4, 11.8, 15.7).
+// Several column tiles a warp once every SM has 32 warps' worth of single ones: four of 16-bit elements, two of FP32. Measured with two / four / eight (us):
+// 14336 x 4096 BF16 30.7 / 25.5 / 24.6 and back 26.8 / 25.4 / 26.9, 2000 x 4096 BF16 5.4 / 5.2 / 6.2 and back 4.2 / 4.2 / 5.1, 2000 x 4096 FP32 6.5 / 6.8 / 7.7
+// and back 6.0 / - / 8.2. 5.8 TB/s of read and written bytes on the first, where the loads' latency is what is left.
 template <typename T>
 constexpr int kBatchOf = sizeof(T) == 4 ? 2 : 4;
 

@@ -22,7 +22,6 @@ constexpr int kWideThreads = 384, kWideEpilogueWarp0 = 4, kWideStages = 6;
 constexpr int kWideStageBytes = kMxTileBytes + kMxQBytes + 2 * kMxSfBytes;
 constexpr int kWideSfCols = 24;  // per stage: 8 TMEM columns of activations' scales, 16 of weights'
 
-
 struct WideParams {
     const uint8_t* W;      // image of the (gate) weights; expert e's lies e * w_expert_bytes behind
     const uint8_t* W_up;
