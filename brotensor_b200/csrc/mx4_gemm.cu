@@ -17,6 +17,7 @@
 // others' shared memory between two cluster barriers a launch took 1.5 us more.)
 //
 // All waits are bounded as in the other kernels; on a timeout the CTA records a status code, sends zeros, frees its TMEM and returns.
+#include <atomic>
 #include <type_traits>
 
 #include "mx4_common.cuh"
@@ -391,6 +392,35 @@ __global__ void __launch_bounds__(kMxThreads<XT>, kIsImage<XT> ? 2 : 3) mx4_gemm
     }
 }
 
+constexpr int mx_budget(int per_sm) { return (per_sm == 3 ? 74 : per_sm == 2 ? 111 : 222) * 1024; }
+
+// CTAs that are resident at a time in clusters of 2^log2 where an SM has room for one: a cluster lies within one group of SMs, which the larger ones do not fill
+// (of 148 SMs clusters of 2 / 4 / 8 take 148 / 132 / 120). One cluster too many is a second wave: 72 rows of 2048 x 8192 in 16 clusters of 8 took 15.5 us, in 16 of 4
+// 11.9; of 4608 x 6144 in 36 of 4 21.0, of 2 16.2. (With two or three CTAs an SM the largest split was the fastest there, 6400 x 8192 and one row 9.2 us for 10.7.)
+static int64_t mx_resident(int log2, int sms) {
+    static std::atomic<int> known[64][4] = {};
+    int dev = 0, n = 0;
+    if (log2 == 0 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms;
+    if ((n = known[dev][log2].load(std::memory_order_relaxed)) != 0) return n;
+    auto kern = mx4_gemm_kernel<1, void>;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 1u << log2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(1u << log2);
+    cfg.blockDim = dim3(kMxThreads<void>);
+    cfg.dynamicSmemBytes = mx_budget(1);
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        return sms;
+    }
+    known[dev][log2].store(n << log2, std::memory_order_relaxed);
+    return n << log2;
+}
+
 template <int MATS, typename XT>
 static int launch_mx_gemm(const MxParams& q, int64_t x_tiles, int64_t rows_most, int sms, cudaStream_t st) {
     auto kern = mx4_gemm_kernel<MATS, XT>;
@@ -418,17 +448,17 @@ static int launch_mx_gemm(const MxParams& q, int64_t x_tiles, int64_t rows_most,
         p.big_bytes = MATS * kMxTileBytes + kMxSfBytes + p.n_cols * 128;
         fixed = (kIsImage<XT> ? 0 : p.split_tiles * x_step) + (split > 1 ? MATS * p.n_cols * 512 : 0);  // activations, parts
         // Shared memory of an SM's `per_sm` CTAs; of fewer where three stages would not fit. The stages' scales take TMEM columns behind the accumulators.
-        budget = per_sm == 3 ? 74 * 1024 : 111 * 1024;
-        if (fixed + 3 * p.stage_bytes > budget) budget = 111 * 1024;
-        if (fixed + 3 * p.stage_bytes > budget || MATS * p.n_cols + 24 * (MATS + 1) > 256) budget = 222 * 1024;
-        // a split whose parts leave an SM room for one CTA only goes as far as there are SMs
-        if (!kIsImage<XT> || split == 1 || budget < 222 * 1024 || tiles * split <= sms) break;
+        budget = mx_budget(per_sm);
+        if (fixed + 3 * p.stage_bytes > budget) budget = mx_budget(2);
+        if (fixed + 3 * p.stage_bytes > budget || MATS * p.n_cols + 24 * (MATS + 1) > 256) budget = mx_budget(1);
+        // a split whose parts leave an SM room for one CTA only goes as far as those are resident
+        if (!kIsImage<XT> || split == 1 || budget < mx_budget(1) || tiles * split <= mx_resident(p.split_log2, sms)) break;
     }
     const int acc = MATS * p.n_cols, sf = 8 * (MATS + 1);
     p.n_stages = (budget - fixed) / p.stage_bytes;
     if (p.n_stages > kMxMaxStages) p.n_stages = kMxMaxStages;
     if (!kIsImage<XT> && p.n_stages > p.split_tiles) p.n_stages = p.split_tiles;
-    const int most = budget == 222 * 1024 ? 512 : 256;
+    const int most = budget == mx_budget(1) ? 512 : 256;
     while (acc + p.n_stages * sf > most) --p.n_stages;
     p.big_stages = p.n_stages * p.stage_bytes / p.big_bytes;  // (three or more of the others, at least one of these)
     p.tmem_cols = 32u;
@@ -444,7 +474,7 @@ static int launch_mx_gemm(const MxParams& q, int64_t x_tiles, int64_t rows_most,
     cudaLaunchConfig_t cfg = {};
     // an image's products: persistent CTAs, whose ring runs on from item to item
     int64_t ctas = tiles * split;
-    const int64_t resident = (int64_t)sms * (budget == 222 * 1024 ? 1 : per_sm);
+    const int64_t resident = (int64_t)sms * (budget == mx_budget(1) ? 1 : per_sm);
     if (kIsImage<XT> && split == 1 && ctas > resident) ctas = resident;
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kMxThreads<XT>);
@@ -507,10 +537,16 @@ int launch_mx4_wide(const void* W, const void* W_up, const void* X, const void* 
 int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* bias, int bias_dtype, void* Y, int y_dtype, int M, int N, int K, const int* plan, int64_t pairs,
                     int E, int early, int sms, int* status, cudaStream_t st) {
     // Where the wide tiles are the faster ones, by measurement (small tiles' time grows with the rows, the wide ones' hardly; us, small and wide):
-    // 14336 x 4096 at 32 / 48 / 64 rows 12.8 13.4 / 15.0 13.3 / 17.1 13.6 - row tiles for every SM, nothing to split -, 4096 x 4096 at 64 / 80 / 128
-    // 9.6 11.6 / 11.8 11.8 / 15.1 12.0, 2560 x 6912 at 64 / 96 / 128 9.7 14.6 / 13.4 14.8 / 15.8 14.8, 1024 x 4096 at 64 / 128 / 256 7.1 10.9 / 10.5 11.3 / 18.5 11.5. Experts, on average 8 / 12 / 16 pairs each:
-    // 128 gated 768 x 2048 40.5 41.8 / 51.5 42.1 / 48.7 42.9, 32 of 2048 x 2048 16.4 19.7 / - / 24.8 19.6, 8 gated 4096 x 4096 27.0 31.6 / - / 32.6 31.7.
-    const bool many = plan ? pairs >= 12LL * E : M >= (mx_row_tiles(N) * 2 > sms ? 48 : 88);
+    // row tiles for every SM, nothing to split: 14336 x 4096 at 32 / 48 / 64 rows 12.7 13.4 / 14.9 13.6 / 16.9 13.6;
+    // too many for a split by four with one CTA an SM, as it is from 65 rows: 8192 x 8192 at 64 / 72 / 87 15.2 16.8 / 18.6 17.0 / 20.3 17.0, 4608 x 4096 at 48 / 72 / 87
+    // 12.3 11.7 / 15.1 11.8 / 16.8 11.8;
+    // fewer: 4096 x 4096 at 64 / 80 / 128 9.6 11.5 / 11.8 11.8 / 15.1 12.0, 1024 x 4096 7.1 10.9 / 8.2 10.9 / 10.4 11.1;
+    // and with many columns, which the wide form does not split: 2560 x 6912 at 80 / 96 / 112 / 128 12.4 14.6 / 13.3 14.7 / 14.6 14.8 / 15.7 14.8, 4096 x 14336 15.6 23.0 /
+    // 16.8 23.1 / 18.0 23.2 / 19.3 23.3, 512 x 7168 8.4 13.9 / 9.1 14.1 / 10.0 14.3 / 10.7 14.4.
+    // Experts, on average 8 / 12 / 16 pairs each: 128 gated 768 x 2048 40.5 41.8 / 51.5 42.1 / 48.7 42.9, 32 of 2048 x 2048 16.4 19.7 / - / 24.8 19.6,
+    // 8 gated 4096 x 4096 27.0 31.6 / - / 32.6 31.7.
+    const int64_t row_tiles = mx_row_tiles(N);
+    const bool many = plan ? pairs >= 12LL * E : M >= (row_tiles * 2 > sms ? 48 : row_tiles * 4 > mx_resident(2, sms) ? 65 : mx_k_tiles(K) >= 24 ? 120 : 88);
     if (g_mx4_wide == 2 || (g_mx4_wide == 1 && many))
         return launch_mx4_wide(W, W_up, X, bias, bias_dtype, Y, y_dtype, M, N, K, plan, pairs, E, early, sms, status, st);
     int64_t x_tiles;

@@ -168,3 +168,12 @@ def test_long_columns_of_few_rows():
         x = _randn((2, K), BF16, 8)
         q = ref.quantise(x)
         _check(ops.mx4_linear(W, x, 130, out_dtype=F32), q @ w[0].T, q.abs() @ w[0].abs().T, K)
+
+
+@pytest.mark.parametrize("M,N,K", [(72, 4608, 2048), (65, 4300, 1056), (72, 2048, 8192), (87, 1700, 8224), (100, 512, 6176), (119, 1000, 6400), (119, 4224, 6144)])
+def test_rows_between_the_two_forms(M, N, K):
+    """Rows of a size where both forms of the product, and splits of different widths, meet: one CTA an SM, whose clusters do not fill them all."""
+    W, w = _weights(N, K, M)
+    x = _randn((M, K), BF16, N)
+    q = ref.quantise(x)
+    _check(ops.mx4_linear(W, x, N, out_dtype=F32), q @ w[0].T, q.abs() @ w[0].abs().T, K)
