@@ -1,5 +1,9 @@
 """MXFP4 products and expert layers where a kernel can go wrong beside its arithmetic: extreme scales, offsets beyond 32 bits, several streams at
 once, launches with and without overlap, weights and plans written by the launch just before."""
+import os
+import subprocess
+import sys
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -177,3 +181,32 @@ def test_rows_between_the_two_forms(M, N, K):
     x = _randn((M, K), BF16, N)
     q = ref.quantise(x)
     _check(ops.mx4_linear(W, x, N, out_dtype=F32), q @ w[0].T, q.abs() @ w[0].abs().T, K)
+
+
+def test_first_calls_of_a_process_are_captured():
+    """What the library asks the device once (attributes, how many clusters it holds) may be asked while a stream is captured."""
+    code = """
+import torch, mx4_reference as ref
+from brotensor_b200 import ops
+N, K = 2048, 8192
+W = ops.mx4_pack(ref.random_blocks(N * (K // 32), 1).cuda().reshape(-1), N, K)
+xs = [torch.randn(M, K, device="cuda") for M in (1, 40, 72, 300)]
+ids = torch.randint(0, 4, (50, 2), dtype=torch.int32, device="cuda")
+E = ops.mx4_pack(ref.random_blocks(4 * 96 * 8, 2).cuda().reshape(-1), 96, 256, count=4)
+def run():
+    plan = ops.moe_plan(ids, 4)
+    return [ops.mx4_linear(W, x, N) for x in xs] + [ops.moe_mx4_linear(E, xs[0][:, :256].expand(50, 256).contiguous(), plan, 96)]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    ys = run()
+g.replay()
+g.replay()
+for a, b in zip(ys, run()):
+    assert torch.equal(a, b)
+assert ops.device_status() == 0
+print("same")
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([os.path.dirname(here), here] + os.environ.get("PYTHONPATH", "").split(os.pathsep)))
+    out = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
