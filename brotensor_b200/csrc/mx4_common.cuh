@@ -63,7 +63,26 @@ inline size_t mx_smem_for_tmem(size_t bytes, uint32_t cols) {
     return bytes < least ? least : bytes;
 }
 
+// A store of 32 bytes came with PTX ISA 8.8, that is CUDA 12.9. An older toolkit's ptxas refuses it; two of 16 bytes write the same.
+#ifndef B200Q_STORE32
+#if __CUDACC_VER_MAJOR__ > 12 || (__CUDACC_VER_MAJOR__ == 12 && __CUDACC_VER_MINOR__ >= 9)
+#define B200Q_STORE32 1
+#else
+#define B200Q_STORE32 0
+#endif
+#endif
+
 #ifdef __CUDACC__
+// 32 bytes to a 32-byte aligned address
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&w)[8]) {
+#if B200Q_STORE32
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+#else
+    static_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    static_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+#endif
+}
 __device__ __forceinline__ float e8m0_to_f32(uint32_t e) {  // 2^(e - 127); 0 is 2^-127, a subnormal
     return e == 255u ? __uint_as_float(0x7FC00000u) : e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23);
 }

@@ -101,9 +101,8 @@ __global__ void __launch_bounds__(kQuantThreads) mx4_dequantise_kernel(const uin
         for (int j = 0; j < 8; ++j) o.e[j] = from_f32<T>(h2f(j & 1 ? h[j >> 1] >> 16 : h[j >> 1] & 0xFFFFu) * d);
         uint4* to = reinterpret_cast<uint4*>(dst + u * kMxTileK);
         if (sizeof(T) == 4 && (reinterpret_cast<uintptr_t>(out) & 31) == 0) {  // whole sectors; two 16-byte stores leave halves
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(o.v[0].x), "r"(o.v[0].y), "r"(o.v[0].z), "r"(o.v[0].w), "r"(o.v[sizeof(T) / 2 - 1].x),
-                         "r"(o.v[sizeof(T) / 2 - 1].y), "r"(o.v[sizeof(T) / 2 - 1].z), "r"(o.v[sizeof(T) / 2 - 1].w)
-                         : "memory");
+            const uint4 lo = o.v[0], hi = o.v[sizeof(T) / 2 - 1];
+            st_global_32(to, {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w});
         } else {
 #pragma unroll
             for (int j = 0; j < (int)(sizeof(T) / 2); ++j) to[j] = o.v[j];

@@ -72,9 +72,7 @@ __device__ __forceinline__ void store16(T* dst, const float (&v)[16], int left, 
         }
 #pragma unroll
         for (int i = 0; i < W; i += 8)
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(dst) + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]),
-                         "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
-                         : "memory");
+            st_global_32(reinterpret_cast<uint32_t*>(dst) + i, {w[i], w[i + 1], w[i + 2], w[i + 3], w[i + 4], w[i + 5], w[i + 6], w[i + 7]});
     } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
