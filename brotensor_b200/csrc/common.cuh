@@ -387,6 +387,34 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// Who arrives at a barrier decides how it is waited for.
+enum MbarWait {
+    kMbarCta,      // this CTA's threads and copies: mbar_try_wait
+    kMbarCluster,  // other CTAs' too, and their data is read behind it: acquire at the cluster's scope (which empties the L1)
+    kMbarOrder,    // other CTAs' too, and nothing but asynchronous work (copies, MMAs, reads of TMEM, with their own fences) has to be in order
+};
+template <MbarWait kWait>
+__device__ __forceinline__ bool mbar_try_wait_as(uint32_t bar, uint32_t parity) {
+    if constexpr (kWait == kMbarCta) return mbar_try_wait(bar, parity);
+    uint32_t ok;
+    if constexpr (kWait == kMbarCluster)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    return ok != 0;
+}
 // Non-blocking probe of a phase (try_wait may park the thread for a hardware time slice).
 __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;

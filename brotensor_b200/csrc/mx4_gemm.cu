@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kMxThreads<XT>, kIsImage<XT> ? 2 : 3) mx4_gemm
                     }
             }
             // (a peer that waits in vain for something gives up before this does)
-            const bool ok = rows > 0 && mx_warp_wait(smem_u32(&bar_parts), 0, &abort_flag, p.status, kDevTimeoutPeer, 4 * kWaitLimitNs);
+            const bool ok = rows > 0 && mx_warp_wait<kMbarCluster>(smem_u32(&bar_parts), 0, &abort_flag, p.status, kDevTimeoutPeer, 4 * kWaitLimitNs);
             if (ok && n < p.N) {
                 for (int t = t0; t < rows; t += split) {
                     float s[MATS];

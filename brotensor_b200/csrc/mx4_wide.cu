@@ -112,6 +112,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
     if (!p.early || warp != 0) grid_dep_wait();
     const uint32_t tmem_base = tmem_base_slot;
 
+    // bar_empty, bar_accum and bar_free are arrived at by the pair's other CTA: commits of MMAs, and "accumulator taken". (Waits that acquire at the cluster's scope empty
+    // the L1: with a bias 99 us for 86.) bar_full is in the first place a CTA's own copies.
     // A unit is two neighbouring activation tiles of one group (or its last one); an item is a unit x a 256-wide tile of weights.
     const int units = p.units ? (int)ld_l2_u32(p.n_units) : (p.M + 2 * kMxTileRows - 1) / (2 * kMxTileRows);
     const int items = units * p.w_tiles;
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
                 if (slot == 0) phase ^= 1;
             }
             for (; kt < p.k_tiles; ++kt) {
-                if (!(ok = mx_warp_wait(smem_u32(&bar_empty[slot]), phase, &abort_flag, p.status, kDevTimeoutEmpty))) break;
+                if (!(ok = mx_warp_wait<kMbarOrder>(smem_u32(&bar_empty[slot]), phase, &abort_flag, p.status, kDevTimeoutEmpty))) break;
                 if (mx_elect()) {
                     load_w(kt, sbase + slot * kWideStageBytes, smem_u32(&bar_full[slot]));
                     load_x(kt, sbase + slot * kWideStageBytes, smem_u32(&bar_full[slot]));
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
             const uint32_t id0 = instr_desc_mxf4(256, 256, 0), id2 = instr_desc_mxf4(256, 256, 2);
             bool ok = true;
             for (int i = worker; ok && i < items; i += workers) {
-                if (!(ok = mx_warp_wait(smem_u32(&bar_free), free_phase, &abort_flag, p.status, kDevTimeoutEmpty))) break;
+                if (!(ok = mx_warp_wait<kMbarOrder>(smem_u32(&bar_free), free_phase, &abort_flag, p.status, kDevTimeoutEmpty))) break;
                 free_phase ^= 1;
                 for (int kt = 0; kt < p.k_tiles; ++kt) {
                     if (!(ok = mx_warp_wait(smem_u32(&bar_full[slot]), phase, &abort_flag, p.status, kDevTimeoutFull))) break;
@@ -263,7 +265,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
             Item it;
             item_of(i, it);
             const int row = r < it.rows ? (p.units ? (int)ld_dep_u32(p.order + it.first + r) : it.first + r) : -1;
-            if (!mx_warp_wait(smem_u32(&bar_accum), phase, &abort_flag, p.status, kDevTimeoutMma)) break;
+            if (!mx_warp_wait<kMbarOrder>(smem_u32(&bar_accum), phase, &abort_flag, p.status, kDevTimeoutMma)) break;
             phase ^= 1;
             tc_fence_after();
             // plain: columns 128 half ..; gated: gate columns 64 half .. in acc[0..63], up columns behind them

@@ -94,12 +94,13 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 // the timer is read only when the thread has to wait.
 // (Measured: the waiting part as a function of its own, not inlined, made every decode GEMV 1 to 10 %
 // slower - a kernel with a call in it gets a worse register allocation around its hot loop.)
+template <MbarWait kWait = kMbarCta>
 __device__ __forceinline__ bool wait_or_abort_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code,
                                                    uint64_t limit_ns) {
     const uint64_t t0 = global_timer_ns();
     for (;;) {
         for (int i = 0; i < 64; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
+            if (mbar_try_wait_as<kWait>(bar, parity)) return true;
         if (*abort_flag) return false;
         if (global_timer_ns() - t0 > limit_ns) {
             *abort_flag = 1;
