@@ -241,9 +241,17 @@ __device__ __forceinline__ bool mx_warp_wait(uint32_t bar, uint32_t parity, vola
     return __all_sync(0xffffffffu, wait_or_abort_slow<kWait>(bar, parity, abort_flag, status, code, limit_ns) && !*abort_flag);
 }
 
-// silu(g) * u. exp2f of a rounded product: |g| 2^-24 off relative, which only negative g feel, where silu is small; the quotient within two units.
+// silu(g) * u = g u / (1 + e^-g), from s = e^(-|g| / 2) <= 1: g / (1 + s s) or, for negative g, g s s / (1 + s s). Nothing leaves the range of the fast exponential and
+// reciprocal. (From e^-g itself the quotient is 0 below g = -87.3, where e^-g passes 2^126; silu(-88) u need not be.) Off by |g| 2^-24 for the rounded argument, which only
+// negative g feel, where silu is small, and 4.5 units of 2^-22: s by 1 twice, the reciprocal by a half, a sum and five products by a quarter each.
 // (expf and a full division are 50 instructions a value: the gated tiles of mx4_wide.cu took 9000 clocks for the 8300 of their products.)
-__device__ __forceinline__ float silu_times(float g, float u) { return __fdividef(g, 1.f + exp2f(-1.4426950408889634f * g)) * u; }
+__device__ __forceinline__ float silu_times(float g, float u) {
+    float s, inv;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(-0.721347520444481704f * fabsf(g)));  // log2(e) / 2
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fmaf(s, s, 1.f)));
+    const float t = g < 0.f ? s : 1.f;
+    return g * t * t * inv * u;
+}
 __device__ __forceinline__ float load_bias(const void* bias, int dtype, size_t i) {
     if (dtype == B200Q_DT_F32) return static_cast<const float*>(bias)[i];
     if (dtype == B200Q_DT_F16) return __half2float(static_cast<const __half*>(bias)[i]);
