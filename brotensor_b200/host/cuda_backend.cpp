@@ -391,7 +391,7 @@ void moe_product(const char* op, const Tensor& image, const Tensor* up, int expe
     check_image(image, experts, out, X.cols, op);
     if (up) check_image(*up, experts, out, X.cols, op);
     const std::size_t bytes = b200q_moe_plan_bytes(tokens, k, experts);
-    if (!bytes || plan.dtype != Dtype::INT32 || plan.bytes() < bytes) op_fail(op, "the plan must be of these tokens, k and experts (moe_route_forward)");
+    if (!bytes || plan.dtype != Dtype::INT32 || plan.bytes() != bytes) op_fail(op, "the plan must be of these tokens, k and experts (moe_route_forward)");
     if (X.rows != tokens && X.rows != tokens * k) op_fail(op, "X must have a row for each token or for each token and choice");
     check_bias(bias, X, experts * out, op);
     size_out(Y, tokens * k, out, X.dtype);
