@@ -339,14 +339,17 @@ void mxfp4_pack_impl(const Tensor& W, int experts, Tensor& image) {
     check_w(W, Dtype::MXFP4, "MXFP4", 32, op);
     if (experts < 1 || W.rows % experts) op_fail(op, "W.rows must be a multiple of the number of experts");
     const std::size_t tiles = b200q_mx4_image_bytes(W.rows / experts, W.cols) / kMxTileBytes * static_cast<std::size_t>(experts);
-    if (tiles * kMxTileBytes > 0x7FFFFFFFull) op_fail(op, "the image is larger than a Tensor holds (2^31 elements): pack fewer experts at a time");
-    const int rows = static_cast<int>(tiles);
-    if (image.rows != rows || image.cols != kMxTileBytes || image.dtype != Dtype::INT8 || !image.data) image.resize(rows, kMxTileBytes, Dtype::INT8);
+    // a Tensor counts its elements in an int: beyond that many bytes the image's rows are counted in words
+    const bool words = tiles * kMxTileBytes > 0x7FFFFFFFull;
+    const int rows = static_cast<int>(tiles), cols = words ? kMxTileBytes / 4 : kMxTileBytes;
+    const Dtype dt = words ? Dtype::INT32 : Dtype::INT8;
+    if (tiles * cols > 0x7FFFFFFFull) op_fail(op, "the image is larger than a Tensor holds (2^31 words of 4 bytes)");
+    if (image.rows != rows || image.cols != cols || image.dtype != dt || !image.data) image.resize(rows, cols, dt);
     check_status(b200q_mx4_pack(W.data, experts, W.rows / experts, W.cols, image.data, cuda_current_stream(W.device.index)), op);
 }
 void check_image(const Tensor& image, int experts, int out, int in, const char* op) {
     if (out < 0 || experts < 1 || in <= 0 || in % 32) op_fail(op, "in must be a multiple of 32, out and experts must not be negative");
-    if (image.dtype != Dtype::INT8 || image.bytes() < static_cast<std::size_t>(experts) * b200q_mx4_image_bytes(out, in))
+    if ((image.dtype != Dtype::INT8 && image.dtype != Dtype::INT32) || image.bytes() < static_cast<std::size_t>(experts) * b200q_mx4_image_bytes(out, in))
         op_fail(op, "the weights must be an image of these matrices (mxfp4_pack)");
 }
 void check_bias(const Tensor* bias, const Tensor& X, int n, const char* op) {

@@ -2,7 +2,7 @@
 // know the format and whose op table has no expert layer; shapes and errors follow the conventions of ops/quant.h.
 //
 // A weight as a file holds it is a Tensor of Dtype::MXFP4 (gguf::File hands out such tensors); the ops take its image, made once by
-// mxfp4_pack: a Tensor of Dtype::INT8 with one row per tile of 128 x 256 elements. Activations are FP32, FP16 or BF16, quantised on the way. Results
+// mxfp4_pack: a Tensor of Dtype::INT8 with one row per tile of 128 x 256 elements; of Dtype::INT32, with as many rows, from 2^31 bytes on, up to 2^31 words (8.6 GB). Activations are FP32, FP16 or BF16, quantised on the way. Results
 // keep a pre-sized FP32 / FP16 / BF16 destination of the right shape, else they are FP16 for FP16 activations and FP32 for the others.
 // Scratch comes from the stream-ordered pool, so that every op may be captured.
 #pragma once

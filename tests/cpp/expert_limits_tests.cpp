@@ -54,6 +54,50 @@ static void test_plan_of_other_sizes() {
     bt::sync(kGpu);
 }
 
+// 31 experts of 16128 x 8192 are an image of 2.18 GB. The first and the last are filled; what they give is what they give on their own.
+static void test_image_beyond_two_gigabytes() {
+    const int E = 31, N = 16128, K = 8192, T = 6;
+    const size_t each = (size_t)N * K / 32 * 17;
+    Tensor W = Tensor::empty_on(kGpu, E * N, K, Dtype::MXFP4), image;
+    CHECK(W.bytes() == E * each);
+    W.zero();
+    Tensor alone[2];
+    for (int i = 0; i < 2; ++i) {
+        const std::vector<uint8_t> b = make_blocks((size_t)N * K / 32, 7 + i);
+        const Tensor part = Tensor::from_raw_bytes_on(kGpu, b.data(), N, K, Dtype::MXFP4, b.size());
+        Tensor here = Tensor::view(kGpu, static_cast<uint8_t*>(W.data) + (i ? (E - 1) * each : 0), N, K, Dtype::MXFP4);
+        here.copy_raw_from_host_async(b.data());
+        bt::sync(kGpu);
+        bt::mxfp4_pack(part, 1, alone[i]);
+        CHECK(alone[i].dtype == Dtype::INT8);
+    }
+    bt::mxfp4_pack(W, E, image);
+    CHECK(image.dtype == Dtype::INT32 && image.cols == 4352 && image.rows == E * 126 * 32 && image.bytes() == E * alone[0].bytes());
+    std::vector<float> x((size_t)T * K), logits((size_t)T * E, 0.f);
+    for (size_t i = 0; i < x.size(); ++i) x[i] = (float)((int)(i * 2654435761u >> 20) - 2048) / 700.f;
+    for (int t = 0; t < T; ++t) logits[(size_t)t * E + (t % 2 ? E - 1 : 0)] = 1.f;
+    const Tensor X = Tensor::from_host_on(kGpu, x.data(), T, K);
+    Tensor ids, weights, plan, Y, A[2];
+    bt::moe_route_forward(Tensor::from_host_on(kGpu, logits.data(), T, E), 1, true, 1.f, ids, weights, plan);
+    bt::moe_linear_forward(image, E, N, nullptr, X, plan, T, 1, Y);
+    for (int i = 0; i < 2; ++i) bt::mxfp4_linear_forward(alone[i], N, nullptr, X, A[i]);
+    bt::sync(kGpu);
+    const std::vector<float> y = Y.to_host_vector(), a[2] = {A[0].to_host_vector(), A[1].to_host_vector()};
+    double off = 0, top = 0;
+    for (int t = 0; t < T; ++t)
+        for (int n = 0; n < N; ++n) {
+            const double want = a[t % 2][(size_t)t * N + n], d = y[(size_t)t * N + n] - want;
+            off += d * d;
+            top += want * want;
+        }
+    CHECK(top > 0 && off < top * 1e-12);  // (sums of another order)
+    // by its numbers alone: a view that claims more than there is
+    const Tensor more = Tensor::view(kGpu, W.data, 1 << 20, 16384, Dtype::MXFP4);
+    Tensor none;
+    CHECK(throws_with([&] { bt::mxfp4_pack(more, 1, none); }, "larger than a Tensor holds"));
+    CHECK(!none.data);
+}
+
 int main(int argc, char** argv) {
     const std::string which = argc > 1 ? argv[1] : "";
     bt::init();
@@ -62,6 +106,7 @@ int main(int argc, char** argv) {
         return 0;
     }
     if (which == "plan") test_plan_of_other_sizes();
+    else if (which == "image") test_image_beyond_two_gigabytes();
     else CHECK(!"the name of a test");
     int st = 0;
     CHECK(b200q_device_status(&st) == B200Q_OK && st == 0);

@@ -18,7 +18,7 @@ def exe():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("which", ["plan"])
+@pytest.mark.parametrize("which", ["plan", "image"])
 def test_expert_limits(exe, which):
     r = subprocess.run([exe, which], capture_output=True, text=True, timeout=300)
     sys.stdout.write(r.stdout[-3000:] + r.stderr[-2000:])
