@@ -27,12 +27,17 @@ static int check_k(const char* op, int K) {
     if (K <= 0 || K % 32) return fail(B200Q_ERR_BAD_ARG, "%s: K (%d) must be a positive multiple of 32", op, K);
     return B200Q_OK;
 }
-// Sizes of a layer of experts; pairs of a token and an expert are numbered in 31 bits, with room for the last tile of each expert.
+// Pairs of a token and an expert are numbered in 31 bits, with room for the last tile of each expert.
+constexpr int64_t kMostPairs = 2147483647LL - (int64_t)kMaxExperts * kMxTileRows;
+static bool experts_fit(int64_t tokens, int k, int E) {
+    return tokens >= 0 && E >= 1 && E <= kMaxExperts && k >= 1 && k <= kMaxExpertsPerToken && tokens <= kMostPairs / k;
+}
+// Sizes of a layer of experts
 static int check_experts(const char* op, int64_t tokens, int k, int E) {
     if (tokens < 0) return fail(B200Q_ERR_BAD_ARG, "%s: negative token count", op);
     if (E < 1 || E > kMaxExperts) return fail(B200Q_ERR_UNSUPPORTED, "%s: E (%d) must be 1..%d", op, E, kMaxExperts);
     if (k < 1 || k > kMaxExpertsPerToken) return fail(B200Q_ERR_UNSUPPORTED, "%s: k (%d) must be 1..%d", op, k, kMaxExpertsPerToken);
-    if (tokens > (2147483647LL - (int64_t)kMaxExperts * kMxTileRows) / k) return fail(B200Q_ERR_UNSUPPORTED, "%s: %lld tokens of %d experts each are too many", op, (long long)tokens, k);
+    if (!experts_fit(tokens, k, E)) return fail(B200Q_ERR_UNSUPPORTED, "%s: %lld tokens of %d experts each are too many", op, (long long)tokens, k);
     return B200Q_OK;
 }
 
@@ -124,7 +129,7 @@ int b200q_mx4_linear(const void* W, const void* X, int x_dtype, const void* bias
 }
 
 size_t b200q_moe_plan_bytes(int64_t tokens, int k, int E) {
-    if (tokens < 0 || k < 1 || k > kMaxExpertsPerToken || E < 1 || E > kMaxExperts) return 0;
+    if (!experts_fit(tokens, k, E)) return 0;
     return 4 * moe_plan_layout(tokens * k, E).total;
 }
 
@@ -151,7 +156,7 @@ int b200q_moe_route(const void* logits, int dtype, int64_t tokens, int E, int k,
 }
 
 size_t b200q_moe_mx4_workspace_bytes(int64_t tokens, int k, int E, int K) {
-    if (tokens < 0 || k < 1 || k > kMaxExpertsPerToken || E < 1 || E > kMaxExperts || K <= 0 || K % 32) return 0;
+    if (!experts_fit(tokens, k, E) || K <= 0 || K % 32) return 0;
     return mx4_dense_takes(tokens * k, K) ? 0 : (size_t)moe_plan_layout(tokens * k, E).max_tiles * mx_k_tiles(K) * kMxTileBytes;
 }
 

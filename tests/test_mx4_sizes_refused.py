@@ -1,0 +1,26 @@
+"""Sizes that no call takes have no size either, and none of them is folded into one that would be taken. (Without a device.)"""
+import pytest
+
+torch = pytest.importorskip("torch")
+from brotensor_b200 import _capi as capi
+from brotensor_b200 import ops
+
+MOST = 2 ** 31 - 1 - 1024 * 128  # pairs
+
+
+@pytest.mark.parametrize("tokens,k", [(MOST + 1, 1), (MOST // 32 + 1, 32), (2 ** 40, 2), (2 ** 62, 4), (2 ** 63 - 1, 32), (2 ** 59, 32)])
+def test_sizes_of_more_pairs_than_a_plan_holds_are_0(tokens, k):
+    L = capi.lib()
+    buf = 1 << 20  # (an aligned address that nothing reads)
+    assert L.b200q_moe_plan(buf, tokens, k, 64, buf, None) == capi.ERR_UNSUPPORTED
+    assert L.b200q_moe_plan_bytes(tokens, k, 64) == 0
+    assert L.b200q_moe_mx4_workspace_bytes(tokens, k, 64, 256) == 0
+    with pytest.raises(ValueError, match="supported sizes"):
+        ops.MoePlan(tokens, k, 64, "meta")
+
+
+@pytest.mark.parametrize("k", [1, 32])
+def test_the_most_pairs_have_a_size(k):
+    L = capi.lib()
+    assert L.b200q_moe_plan_bytes(MOST // k, k, 1024) > 8 * (MOST // k) * k
+    assert L.b200q_moe_mx4_workspace_bytes(MOST // k, k, 1024, 256) >= (MOST // k * k // 128) * 17408
