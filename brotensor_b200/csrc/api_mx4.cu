@@ -55,6 +55,7 @@ int b200q_mx4_pack(const void* blocks, int64_t count, int64_t rows, int K, void*
     if (rows == 0 || count == 0) return B200Q_OK;
     if (!blocks || !image) return fail(B200Q_ERR_BAD_ARG, "mx4_pack: null pointer");
     if (!on(image, 16)) return fail(B200Q_ERR_BAD_ARG, "mx4_pack: the image must be 16-byte aligned");
+    if (rows > 8 * 2147483647LL / count) return fail(B200Q_ERR_UNSUPPORTED, "mx4_pack: %lld x %lld rows are more than one launch takes", (long long)count, (long long)rows);
     int sms, *status;
     if (int rc = device_facts(&sms, &status)) return rc;
     return launch_mx4_pack(blocks, rows, count, K, image, static_cast<cudaStream_t>(stream));

@@ -24,3 +24,10 @@ def test_the_most_pairs_have_a_size(k):
     L = capi.lib()
     assert L.b200q_moe_plan_bytes(MOST // k, k, 1024) > 8 * (MOST // k) * k
     assert L.b200q_moe_mx4_workspace_bytes(MOST // k, k, 1024, 256) >= (MOST // k * k // 128) * 17408
+
+
+@pytest.mark.parametrize("count,rows", [(2 ** 32, 2 ** 32 + 1), (2 ** 62, 4), (2 ** 63 - 1, 3), (1, 2 ** 34), (2 ** 34, 1)])
+def test_pack_of_more_rows_than_64_bits_count(count, rows):
+    buf = 1 << 20
+    L = capi.lib()
+    assert L.b200q_mx4_pack(buf, count, rows, 32, buf, None) == capi.ERR_UNSUPPORTED and b"more than one launch" in L.b200q_last_error()
