@@ -432,6 +432,8 @@ def moe_combine(y: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, exper
     T, k, N = y.shape
     if k >> 31 or N >> 31 or experts >= 1 << 31:
         raise ValueError(f"k ({k}), N ({N}) and experts ({experts}) must be below 2^31")
+    if experts < 1:
+        raise ValueError(f"experts ({experts}) must be positive")
     device, code, pairs = y.get_device(), _DT.get(y.dtype), (T, k)
     if (code is None or device < 0 or ids.dtype is not torch.int32 or weights.dtype is not torch.float32 or ids.shape != pairs or weights.shape != pairs
             or ids.get_device() != device or weights.get_device() != device or not (y.is_contiguous() and ids.is_contiguous() and weights.is_contiguous())):

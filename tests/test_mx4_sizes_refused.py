@@ -31,3 +31,10 @@ def test_pack_of_more_rows_than_64_bits_count(count, rows):
     buf = 1 << 20
     L = capi.lib()
     assert L.b200q_mx4_pack(buf, count, rows, 32, buf, None) == capi.ERR_UNSUPPORTED and b"more than one launch" in L.b200q_last_error()
+
+
+@pytest.mark.parametrize("experts", [0, -1, -2 ** 31 - 1, -2 ** 32 + 4])
+def test_sum_over_no_experts(experts):
+    """ctypes would pass the low 32 bits on: -2^32 + 4 are 4 experts."""
+    with pytest.raises(ValueError, match="experts"):
+        ops.moe_combine(torch.empty(1, 2, 8, device="meta"), torch.empty(1, 2, dtype=torch.int32, device="meta"), torch.empty(1, 2, device="meta"), experts)
