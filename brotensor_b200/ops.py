@@ -405,7 +405,8 @@ def _moe_common(Ws, X, plan, N, out, out_dtype, ws):
 
 def moe_mx4_linear(W, X, plan: MoePlan, N: int, bias=None, out=None, out_dtype=None, ws=None) -> torch.Tensor:
     """out[t][j] = quantise(X[t] or X[t][j]) @ W[e].T (+ bias[e]), e the j-th expert of token t: (tokens, k, N). W: the
-    experts' images, one after the other. Rows of pairs without an expert are left as they were."""
+    experts' images, one after the other. Rows of pairs without an expert are left as they were: in an `out` made here they hold
+    whatever the memory held (moe_combine and a further product do not read them; other operations would)."""
     code, per_pair, out, K, (ws_ptr, ws_bytes, ws) = _moe_common((W,), X, plan, N, out, out_dtype, ws)
     bias_ptr = None
     if bias is not None:
@@ -418,7 +419,7 @@ def moe_mx4_linear(W, X, plan: MoePlan, N: int, bias=None, out=None, out_dtype=N
 
 
 def moe_mx4_swiglu(W_gate, W_up, X, plan: MoePlan, N: int, out=None, out_dtype=None, ws=None) -> torch.Tensor:
-    """silu(gate) * up of the two products, without writing them out."""
+    """silu(gate) * up of the two products, without writing them out. Rows of pairs without an expert: as moe_mx4_linear."""
     code, per_pair, out, K, (ws_ptr, ws_bytes, ws) = _moe_common((W_gate, W_up), X, plan, N, out, out_dtype, ws)
     capi.check(_launch(X, capi.lib().b200q_moe_mx4_swiglu, W_gate.data_ptr(), W_up.data_ptr(), X.data_ptr(), code, per_pair, plan.data.data_ptr(),
                        out.data_ptr(), _DT[out.dtype], plan.tokens, plan.k, plan.experts, N, K, ws_ptr, ws_bytes))

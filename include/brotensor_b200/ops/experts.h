@@ -20,7 +20,7 @@ void mxfp4_linear_forward(const Tensor& image, int out, const Tensor* bias, cons
 // over the chosen (normalize) or over all experts, times scale; plan: INT32, the grouping of the T * k pairs by expert.
 void moe_route_forward(const Tensor& logits_TE, int k, bool normalize, float scale, Tensor& ids, Tensor& weights, Tensor& plan);
 // Y (T * k, out): row t * k + j is token t's row of X through its j-th expert. X: (T, in), or (T * k, in) with a row for each pair. Rows of pairs without
-// an expert are left as they were. bias: (experts, out) of X's dtype or nullptr.
+// an expert are left as they were (uninitialised where Y is made or resized here; moe_combine_forward and a further product do not read them). bias: (experts, out) of X's dtype or nullptr.
 void moe_linear_forward(const Tensor& image, int experts, int out, const Tensor* bias, const Tensor& X, const Tensor& plan, int tokens, int k, Tensor& Y);
 // silu(gate) * up of two such products
 void moe_swiglu_forward(const Tensor& gate_image, const Tensor& up_image, int experts, int out, const Tensor& X, const Tensor& plan, int tokens, int k, Tensor& Y);
