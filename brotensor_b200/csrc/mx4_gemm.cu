@@ -94,8 +94,8 @@ __global__ void __launch_bounds__(kMxThreads<XT>, kIsImage<XT> ? 2 : 3) mx4_gemm
     if (warp == 1) {
         tmem_alloc(smem_u32(&tmem_base_slot), p.tmem_cols);
         tmem_relinquish();
+        grid_dep_launch();  // not before: a dependent that had taken the columns would wait for this CTA, and this CTA for the columns
     }
-    grid_dep_launch();
     // The L2 hears about the first weights while the predecessor still runs. Whose they are in a grouped product the plan says, which the predecessor
     // may be writing: a hint may be wrong, so it is only checked to lie inside the weights.
     if (warp == 0 && n_kt > 0 && !p.early) {

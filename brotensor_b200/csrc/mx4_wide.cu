@@ -103,8 +103,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) mx4_wide_kernel(const WidePar
         mbar_init(smem_u32(&bar_free), 16);
         fence_mbar_init();
     }
-    if (warp == 1) wide_alloc(smem_u32(&tmem_base_slot));
-    grid_dep_launch();
+    if (warp == 1) {
+        wide_alloc(smem_u32(&tmem_base_slot));
+        grid_dep_launch();  // not before: see mx4_gemm.cu
+    }
     tc_fence_before();
     __syncthreads();
     mx_cluster_sync();

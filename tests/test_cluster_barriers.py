@@ -31,3 +31,13 @@ def test_arrivals():
             assert asm.startswith("mbarrier.arrive.relaxed.cluster."), (name, asm)
     text = _source("common.cuh")
     assert "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64" in text and "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64" in text
+
+
+@pytest.mark.parametrize("name,alloc", [("mx4_gemm.cu", "tmem_alloc"), ("mx4_wide.cu", "wide_alloc")])
+def test_dependents_are_let_go_behind_the_allocation(name, alloc):
+    """A kernel that follows may start from then on. Had it taken the tensor memory's columns first, it would wait for this kernel's end and this kernel for the columns."""
+    text = _source(name)
+    body = text[text.index("__launch_bounds__"):]
+    assert body.count("grid_dep_launch()") == 1
+    block = re.search(r"if \(warp == 1\) \{\s*" + alloc + r"\(([^{}]*)\}", body)
+    assert block and "grid_dep_launch();" in block.group(0)
