@@ -55,11 +55,14 @@ inline __host__ MoePlanLayout moe_plan_layout(int64_t pairs, int E) {
     return l;
 }
 
-// Shared memory that a kernel with `cols` TMEM columns asks for, its own need being `bytes`: at least 456 bytes a column with the 2 KB of
-// static and reserved memory, so that CTAs which an SM takes by its 228 KB always find their columns too, whichever of these kernels
-// share it. (A CTA that waits for columns while its cluster's others hold theirs could otherwise wait for a CTA that waits for it.)
-inline size_t mx_smem_for_tmem(size_t bytes, uint32_t cols) {
-    const size_t least = (size_t)cols * 456 - 2048;
+// Shared memory that a kernel with `cols` TMEM columns asks for, its own need being `bytes`: enough that the CTAs of clusters which an SM takes by its 228 KB always find their
+// columns too, whichever of these kernels share it and whatever has come and gone. (A CTA that waits for columns while its cluster's others hold theirs could otherwise wait for
+// a CTA that waits for it; one of no cluster comes to its end by itself.) 456 bytes a column, with the 2 KB of static and reserved memory, keep the sum at 512. Columns lie at
+// multiples of their number, so that two CTAs of few could keep a third from its 256: 58 KB is more than half of what one of 256 leaves. (Without a cluster there may be more
+// of them: 128256 x 512, one row, 10.7 us, with 58 KB each 12.9.)
+inline size_t mx_smem_for_tmem(size_t bytes, uint32_t cols, bool cluster) {
+    size_t least = (size_t)cols * 456 - 2048;
+    if (cluster && least < 58 * 1024) least = 58 * 1024;
     return bytes < least ? least : bytes;
 }
 

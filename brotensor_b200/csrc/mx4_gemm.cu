@@ -468,7 +468,7 @@ static int launch_mx_gemm(const MxParams& q, int64_t x_tiles, int64_t rows_most,
     p.big_stages = p.n_stages * p.stage_bytes / p.big_bytes;
     p.tmem_cols = 32u;
     while ((int)p.tmem_cols < acc + p.n_stages * sf) p.tmem_cols *= 2;
-    const size_t smem = mx_smem_for_tmem((size_t)p.n_stages * p.stage_bytes + fixed + 1024, p.tmem_cols);
+    const size_t smem = mx_smem_for_tmem((size_t)p.n_stages * p.stage_bytes + fixed + 1024, p.tmem_cols, split > 1);
     static bool configured[64] = {};
     int dev = 0;
     B200Q_CUDA_TRY(cudaGetDevice(&dev));
